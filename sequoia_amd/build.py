@@ -16,7 +16,10 @@ SOURCES = ["kv_ops.hip", "sampler.hip", "verify.hip", "tree_attention.hip", "fus
 PROBES = os.environ.get("SEQUOIA_BUILD_PROBES", "0") == "1"
 if PROBES:
     SOURCES = SOURCES + ["ts_probe.hip", "draft_fused.hip"]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wno-unused-value"] + (["-DSEQUOIA_BUILD_PROBES"] if PROBES else [])
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wno-unused-value",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + (["-DSEQUOIA_BUILD_PROBES"] if PROBES else [])
+# (-packed-fp32-ops: no v_pk_{add,mul,fma}_f32 -- some of their forms have given wrong results now and then; the host pass warns that
+# it does not know the feature)
 # per-source additions.  ts_linear: keep the MFMA accumulators in VGPRs -- with the AGPR form the register
 # allocator permutes the 48-128 accumulator registers on every trip of the ring loop (72 v_accvgpr_* moves
 # per 48 MFMAs in the ISA)
