@@ -33,6 +33,10 @@ extern "C" {
 #define SQ_EUNSUPPORTED -2   /* shape outside what the kernels are built for               */
 #define SQ_ELAUNCH      -3   /* HIP reported an error at launch; see sq_last_error()        */
 
+#define SQ_DTYPE_F16     0   /* element type of the entry points that take more than fp16    */
+#define SQ_DTYPE_BF16    1
+#define SQ_DTYPE_F32     2
+
 #define SQ_MAX_TREE      512 /* max tree nodes (ancestor bitmask = 8 x u64 words)           */
 #define SQ_MASK_WORDS(n) (((n) + 63) / 64)
 #define SQ_MAX_TOPK      128 /* max children per parent / samples per row                   */
@@ -513,6 +517,64 @@ int sq_level_attention_f16(const void* qkv, const float* qkv_slab, int splits, i
                            const int64_t* d_position_ids, const int64_t* d_storage_ids, int q_len, int n_heads, int h_kv, int d,
                            int m, float scale, int q_slot0, int gt, int n_tree, const uint64_t* d_bitmask, int words,
                            const int32_t* d_ctx, void* stream);
+
+/* ---- batched speculative decoding over a paged KV cache --------------------------------------------------------------
+ * One step of a ragged batch: sequence b holds d_seq_lens[b] stored rows and brings rows [d_cu_rows[b], d_cu_rows[b + 1]) of
+ * the batch's new tokens (d_cu_rows[0] = 0, ascending, n_seqs + 1 entries; a sequence may bring none; rows behind the last
+ * sequence -- a padded batch -- are left alone).  A layer's pages are [n_pages][H_kv][page_size][D], page_size 16 / 32 / 64 /
+ * 128 / 256, D 64 / 128; row j of sequence b lives in page d_page_table[b * table_width + j / page_size].  Elements are fp16 or
+ * bf16 (dtype), the same for rows, tables of cosines and outputs; with k_scales and v_scales ([n_pages][H_kv][page_size] bytes)
+ * the pages hold e4m3 codes (OCP, [n_pages][H_kv][page_size][D] bytes) and a row's value is code * 2^(byte - 127).
+ * Lengths, offsets and tables are read on the device: one captured launch serves every step whose host-side bounds hold.  A
+ * page number outside the pool is never followed: rows there are not written or read back, and as keys they are undefined.
+ * Pages that new rows land in belong to one sequence each (two rows written to one place: one of them, or parts of both, stay).
+ */
+
+/* RoPE of packed q | k | v rows and the write of K and V (what sq_rope_kv_write_f16 does for the static slab): q_out is
+ * [H][n_rows][D]; the rotation is computed in fp32 and rounded once, to the stored type.  e4m3: a row's byte is the smallest
+ * >= 1 with largest magnitude / 2^(byte - 127) <= 448, codes round to nearest even; magnitudes stop at 61440 (fp16) or
+ * 1.875 * 2^127 (bf16), an element that is not finite is stored as NaN and has no part in the scale.
+ * cos / sin: [max_pos][D]; position ids outside it are brought to its ends.  16-byte alignment of all rows.             */
+int sq_rope_kv_write_paged(const void* qkv, int64_t qkv_stride, void* q_out, void* k_pages, void* v_pages, void* k_scales,
+                           void* v_scales, const void* cos_tab, const void* sin_tab, int max_pos,
+                           const int64_t* d_position_ids, const int32_t* d_page_table, int table_width, int n_pages,
+                           int page_size, const int32_t* d_seq_lens, const int32_t* d_cu_rows, int n_seqs, int n_rows,
+                           int n_heads, int h_kv, int d, int dtype, void* stream);
+
+/* Stored rows [d_starts[b], d_starts[b] + d_counts[b]) of every sequence into rows [0, d_counts[b]) of
+ * k_out / v_out [n_seqs][H_kv][out_rows][D] (strides in elements; a static slab's layer fits), at most max_count and out_rows of
+ * them; other rows of the outputs stay as they are.  e4m3 rows come back as the values they stand for.                  */
+int sq_kv_read_paged(const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, void* k_out,
+                     void* v_out, int64_t out_seq_stride, int64_t out_head_stride, int out_rows,
+                     const int32_t* d_page_table, int table_width, int n_pages, int page_size, const int32_t* d_starts,
+                     const int32_t* d_counts, int n_seqs, int max_count, int h_kv, int d, int dtype, void* stream);
+
+/* Attention of the new tokens (their own rows written before): row i of sequence b sees keys [0, d_seq_lens[b] + i];
+ * out [n_rows][H * D] (row stride out_stride) = softmax(scale * q k^T) v, sums in fp32.  q: element (head, row, 0) at
+ * head * q_head_stride + row * q_row_stride.  max_rows / max_len: no sequence brings more rows / sees more keys (they size the
+ * launch; rows and keys beyond them are left out).  A row that sees nothing is zeros.  scale > 0.
+ * workspace: sq_paged_attention_workspace_bytes bytes (may be 0), free again when the call's work on the stream is done.  */
+size_t sq_paged_attention_workspace_bytes(int n_seqs, int n_rows, int max_rows, int max_len, int n_heads, int h_kv, int d);
+int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t q_row_stride, const void* k_pages, const void* v_pages,
+                       const void* k_scales, const void* v_scales, void* out, int64_t out_stride,
+                       const int32_t* d_page_table, int table_width, int n_pages, int page_size, const int32_t* d_seq_lens,
+                       const int32_t* d_cu_rows, int n_seqs, int n_rows, int max_rows, int max_len, int n_heads, int h_kv,
+                       int d, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Verification of a batch's drafted tokens.  Sequence b drafted tokens [d_cu_drafts[b], d_cu_drafts[b + 1]); target row
+ * d_cu_drafts[b] + b + i judges its token i, the row behind its last one follows (target_logits: >= n_drafts + n_seqs rows,
+ * draft_logits: >= n_drafts, fp16 / bf16 / fp32).  With p = softmax(target / T), q = softmax(draft / T): tokens are accepted
+ * while u_accept[token] * q(token) < p(token); next = the first token whose running mass of max(p - q, 0) (of p behind the last
+ * drafted token, and where p is nowhere above q) exceeds u_next[b] times its total.  d_temperature[b] (NULL: `temperature`)
+ * = 0: greedy, p is the first maximum.  d_n_accepted[b] = accepted tokens; d_next_tokens[b] = -1 where the deciding row is no
+ * distribution (NaN, +inf, or nothing above -inf).  A drafted token outside the vocabulary is never accepted.  Sums, probabilities and
+ * running masses are 64-bit.                                                                                           */
+size_t sq_verify_drafts_workspace_bytes(int n_seqs, int n_drafts, int vocab);
+int sq_verify_drafts(const void* target_logits, int64_t ld_target, const void* draft_logits, int64_t ld_draft,
+                     const int64_t* d_draft_tokens, const int32_t* d_cu_drafts, int n_seqs, int n_drafts, int vocab,
+                     const float* d_u_accept, const float* d_u_next, const float* d_temperature, float temperature,
+                     int32_t* d_n_accepted, int64_t* d_next_tokens, int dtype, void* workspace, size_t workspace_bytes,
+                     void* stream);
 
 #ifdef __cplusplus
 }

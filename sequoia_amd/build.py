@@ -10,7 +10,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libsequoia_hip.so")
-SOURCES = ["kv_ops.hip", "sampler.hip", "verify.hip", "tree_attention.hip", "fused_ops.hip", "ts_linear.hip", "allreduce.hip", "draft_block.hip"]
+SOURCES = ["kv_ops.hip", "sampler.hip", "verify.hip", "tree_attention.hip", "fused_ops.hip", "ts_linear.hip", "allreduce.hip", "draft_block.hip",
+           "paged_kv.hip", "paged_attention.hip", "verify_drafts.hip"]
 # measurement aids (tools/prefetch_probe.py) and measured-negative experiments (draft_fused.hip: RMSNorm inside the projection,
 # profiles/r03_draft_fused_not_adopted.md) stay out of the product library: SEQUOIA_BUILD_PROBES=1 adds them
 PROBES = os.environ.get("SEQUOIA_BUILD_PROBES", "0") == "1"
@@ -43,7 +44,7 @@ def _stale(target: str, deps: list[str]) -> bool:
 def build(force: bool = False, verbose: bool = True) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     srcs = [os.path.join(CSRC, s) for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
-    hdrs = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "attn_map.h"), os.path.join(os.path.dirname(PKG), "include", "sequoia_hip.h")]
+    hdrs = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "attn_map.h"), os.path.join(CSRC, "paged.h"), os.path.join(os.path.dirname(PKG), "include", "sequoia_hip.h")]
     objs = []
     cc = hipcc()
     for s in srcs:

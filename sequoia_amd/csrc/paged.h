@@ -1,0 +1,77 @@
+// Shared by the paged-cache kernels (paged_kv.hip, paged_attention.hip): element types, page geometry, e4m3 rows.
+//
+// A layer's pages are [n_pages][H_kv][P][D], P a power of two from 16 to 256: a page of a KV head is the same [rows][D] block as
+// the static slab, so a 16-row tile of keys never straddles two pages.  Row j of sequence b lives in page
+// table[b][j >> shift], row j & (P - 1).
+//
+// An e4m3 row keeps one exponent byte x: value = code * 2^(x - 127).  The scale is a power of two so that both directions are
+// exact but for the ONE rounding to e4m3's four significant bits (at most 2^-4 relative, 2^(x - 137) absolute below the
+// format's normal range): x / scale and code * scale never round, and every reader gets the same value.
+#pragma once
+#include "common.h"
+
+typedef __bf16 bf16_t;
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+typedef __bf16 bf4v __attribute__((ext_vector_type(4)));
+typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <typename T> struct vec_of;
+template <> struct vec_of<half_t> { typedef half8 v8; typedef half4 v4; typedef half2v v2; };
+template <> struct vec_of<bf16_t> { typedef bf8v v8; typedef bf4v v4; typedef bf2v v2; };
+
+struct PageMap {
+    const int32_t* table;       // [n_seqs][width]
+    int width, n_pages, shift;  // P = 1 << shift
+};
+
+// page of block `i` of sequence `b`, or -1 where the table holds none: an entry outside the pool is never followed
+__device__ __forceinline__ int page_of(const PageMap& M, int b, int i) {
+    if ((unsigned)i >= (unsigned)M.width) return -1;
+    const int p = M.table[(size_t)b * M.width + i];
+    return (unsigned)p < (unsigned)M.n_pages ? p : -1;
+}
+
+static inline int page_shift(int page_size) {
+    for (int s = 4; s <= 8; ++s)
+        if (page_size == 1 << s) return s;
+    return -1;
+}
+
+// the sequence that row `t` of a ragged batch belongs to (n_seqs: none), by one wave: cu_rows is ascending, so it is the number
+// of sequences that end at or before t.  64 ends a load instead of a search's chain of dependent ones.
+__device__ __forceinline__ int seq_of_row(const int32_t* cu_rows, int n_seqs, int t) {
+    const int lane = threadIdx.x & 63;
+    int seq = 0;
+    for (int base = 0; base < n_seqs; base += 64) {
+        const int i = base + lane;
+        const bool done = i < n_seqs && cu_rows[i + 1] <= t;
+        const int n = __popcll(__ballot(done));
+        seq += n;
+        if (n < 64) break;
+    }
+    return seq;
+}
+
+// 16 codes -> 16 values of T, exact: v_cvt_scalef32 multiplies by the power of two while it widens
+template <typename T>
+__device__ __forceinline__ void e4m3_expand(u32x4 codes, float scale, typename vec_of<T>::v8& lo, typename vec_of<T>::v8& hi) {
+    typename vec_of<T>::v2 p[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (__is_same(T, half_t)) {
+            p[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], scale, false);
+            p[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], scale, true);
+        } else {
+            p[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i], scale, false);
+            p[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i], scale, true);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        lo[2 * i] = p[i][0]; lo[2 * i + 1] = p[i][1];
+        hi[2 * i] = p[4 + i][0]; hi[2 * i + 1] = p[4 + i][1];
+    }
+}
+// exponent byte -> scale; the writer's bytes lie in [1, 254]
+__device__ __forceinline__ float e4m3_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }

@@ -1,0 +1,407 @@
+// Attention of a ragged batch's new tokens over a paged KV cache (their own rows already written): for sequence b with `past`
+// stored rows and n new ones, row i attends keys [0, past + i],
+//     o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   s_j = scale * q . k_j,
+// in one pass over the keys with a running maximum and sum in fp32; weights are rounded to the element type once, for the
+// second matrix product.  The query heads that share a KV head are packed into the same rows of a tile (row r = token r / group,
+// head r % group), so that every stored row is read once for all of them.
+#include "paged.h"
+#include "attn_map.h"
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __fp16 fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
+
+struct PagedAttnParams {
+    const void* q; int64_t q_head_stride, q_row_stride;
+    const void *k, *v;
+    const uint8_t *ks, *vs;
+    void* out; int64_t out_stride;
+    PageMap map;
+    const int32_t *seq_lens, *cu_rows;
+    int n_seqs, n_rows, n_heads, h_kv, group;
+    float scale_log2e;
+    int max_len;                           // no sequence's keys go further (host's bound: the parts cover it)
+    int n_tiles, n_splits, split_len;      // row tiles a (sequence, KV head), parts of the key axis, keys a part
+    float* part_o;                         // [n_splits][n_rows * n_heads][D]: unnormalised
+    float* part_ml;                        // [n_splits][n_rows * n_heads][2]: maximum (log2 units), sum
+};
+
+template <typename T> __device__ __forceinline__ floatx4 mfma16(typename vec_of<T>::v8 a, typename vec_of<T>::v8 b, floatx4 c) {
+    if constexpr (__is_same(T, half_t)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// column (lane & 15) of the 4 x 16 block of 16-bit values whose row (lane & 15) >> 2, columns 4 (lane & 3).. this lane addresses
+__device__ __forceinline__ u32x2 read_transposed(const void* p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)p));
+}
+
+// elements of v that are not finite, as 0; of class c (0: +inf, 1: -inf, 2: NaN), as 1 and the others as 0
+template <typename V8> __device__ __forceinline__ V8 finite_part(V8 v) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __builtin_fabsf((float)v[j]) < INFINITY ? v[j] : 0;
+    return v;
+}
+template <typename V8> __device__ __forceinline__ V8 class_part(V8 v, int c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float x = (float)v[j];
+        v[j] = (c == 0 ? x == INFINITY : c == 1 ? x == -INFINITY : x != x) ? 1 : 0;
+    }
+    return v;
+}
+
+// what a workgroup works on
+struct AttnItem {
+    int seq, kvh, past, rows, first, row0, end, split, n_parts;   // packed rows of the (sequence, KV head), cu_rows[seq], first row, key end
+};
+__device__ __forceinline__ int attn_tile_end(const PagedAttnParams& P, int past, int rows, int tile, int tile_rows) {
+    int last = (tile + 1) * tile_rows;
+    last = last < rows ? last : rows;
+    const int end = past + (last - 1) / P.group + 1;
+    return end < P.max_len ? (end > 0 ? end : 0) : P.max_len;
+}
+// (sequence, KV head) fastest: a multiple of 8 of them keeps all tiles of one in one XCD's L2; the longest tiles start first
+__device__ __forceinline__ bool attn_item(const PagedAttnParams& P, int tile_rows, AttnItem& I) {
+    const int units = P.n_seqs * P.h_kv, u = blockIdx.x % units, w = blockIdx.x / units;
+    I.seq = u / P.h_kv; I.kvh = u - I.seq * P.h_kv;
+    const int tile = P.n_tiles - 1 - w / P.n_splits;
+    I.split = w % P.n_splits;
+    I.first = P.cu_rows[I.seq];
+    int n = P.cu_rows[I.seq + 1] - I.first;
+    if (I.first < 0 || I.first + n > P.n_rows) return false;
+    I.rows = n * P.group;
+    I.row0 = tile * tile_rows;
+    if (I.row0 >= I.rows) return false;
+    I.past = P.seq_lens[I.seq];
+    I.end = attn_tile_end(P, I.past, I.rows, tile, tile_rows);
+    I.n_parts = (I.end + P.split_len - 1) / P.split_len;
+    return I.split < I.n_parts || (I.split == 0 && I.n_parts == 0);
+}
+
+// Few rows (a decoding step, a drafted chunk): bound by the bytes of K and V.  Four waves walk the 32-key chunks of the
+// workgroup's part in turn, each with its own running softmax, and join through LDS.  A chunk is fetched as whole rows (16 bytes
+// a lane, next chunk in flight while this one is computed), staged in the wave's own LDS and read back as
+//   S^T = K Q^T    A = K rows, B = Q: a lane holds 8 scores of one query row, in the order the second product wants them
+//   O^T += V^T P^T A = V^T (transposing LDS reads), B = P^T straight from the registers S^T left behind.
+#define PAD_NW 4
+#define PAD_BK 32
+template <typename T, int D, bool Q8, int MT>
+__global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(PagedAttnParams P) {
+    typedef typename vec_of<T>::v8 v8;
+    typedef typename vec_of<T>::v4 v4;
+    constexpr int EPL = Q8 ? 16 : 8, LPR = D / EPL, RPP = 64 / LPR, PASSES = PAD_BK / RPP;   // elements a lane, lanes a row, rows a pass
+    constexpr int DSTEPS = D / 32, NT = D / 16, ROWS = 16 * MT;
+    constexpr int KSTR = D + 8, VSTR = D + 16;      // 16-byte reads of 16 rows, 8-byte transposing reads of 8 rows: all banks once
+    constexpr int WAVE_BYTES = PAD_BK * (KSTR + VSTR) * 2, OSTR = D + 4;
+    constexpr int LDS_BYTES = PAD_NW * (WAVE_BYTES > ROWS * OSTR * 4 ? WAVE_BYTES : ROWS * OSTR * 4);
+    __shared__ __attribute__((aligned(16))) unsigned char lds[LDS_BYTES];
+    __shared__ float lds_ml[PAD_NW][ROWS][2];
+    AttnItem I;
+    if (!attn_item(P, ROWS, I)) return;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, qc = lane & 15, g = lane >> 4;
+    const int k0 = I.split * P.split_len, k1 = I.end < k0 + P.split_len ? I.end : k0 + P.split_len;
+    T* my_k = (T*)(lds + wave * WAVE_BYTES);
+    T* my_v = my_k + PAD_BK * KSTR;
+
+    v8 qf[MT][DSTEPS];
+    int lim[MT];                                    // last key this lane's query row sees
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        int r = I.row0 + 16 * mt + qc;
+        r = r < I.rows ? r : I.rows - 1;
+        const int token = r / P.group, head = I.kvh * P.group + r - token * P.group;
+        lim[mt] = I.past + token;
+        const T* qr = (const T*)P.q + head * P.q_head_stride + (size_t)(I.first + token) * P.q_row_stride + 8 * g;
+#pragma unroll
+        for (int s = 0; s < DSTEPS; ++s) qf[mt][s] = *(const v8*)(qr + 32 * s);
+    }
+    const int lim0 = I.past + I.row0 / P.group;     // keys up to here are seen by every row of the tile
+
+    float m_run[MT], l_run[MT];
+    floatx4 o_acc[MT][NT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        m_run[mt] = -INFINITY; l_run[mt] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o_acc[mt][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    u32x4 kr[PASSES], vr[PASSES];
+    uint32_t ksr[PASSES], vsr[PASSES];
+    const int lrow = lane / LPR, lcol = lane % LPR;
+    // pages of the two 16-row halves of a chunk; a missing one (only behind a table that ends early) reads page 0, in bounds
+    auto pages = [&](int key0, int& a, int& b) {
+        a = page_of(P.map, I.seq, key0 >> P.map.shift);
+        b = page_of(P.map, I.seq, (key0 + 16) >> P.map.shift);
+        a = a < 0 ? 0 : a; b = b < 0 ? 0 : b;
+    };
+    auto load = [&](int key0, int pa, int pb) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int rr = i * RPP + lrow;
+            const size_t r = (((size_t)(i * RPP < 16 ? pa : pb) * P.h_kv + I.kvh) << P.map.shift) + ((key0 + rr) & ((1 << P.map.shift) - 1));
+            const size_t at = r * D * (Q8 ? 1 : 2) + 16 * lcol;
+            kr[i] = *(const u32x4*)((const uint8_t*)P.k + at);
+            vr[i] = *(const u32x4*)((const uint8_t*)P.v + at);
+            if constexpr (Q8) { ksr[i] = P.ks[r]; vsr[i] = P.vs[r]; }
+        }
+    };
+    int key0 = k0 + wave * PAD_BK, pa = 0, pb = 0;
+    if (key0 < k1) {
+        pages(key0, pa, pb);
+        load(key0, pa, pb);
+        if (key0 + PAD_NW * PAD_BK < k1) pages(key0 + PAD_NW * PAD_BK, pa, pb);
+    }
+    for (; key0 < k1; key0 += PAD_NW * PAD_BK) {
+        const bool tail = key0 + PAD_BK > k1;       // rows behind the end hold anything: their weights are 0, and so are they
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int rr = i * RPP + lrow;
+            if constexpr (Q8) {
+                v8 lo, hi;
+                e4m3_expand<T>(kr[i], e4m3_scale(ksr[i]), lo, hi);
+                *(v8*)(my_k + rr * KSTR + 16 * lcol) = lo;
+                *(v8*)(my_k + rr * KSTR + 16 * lcol + 8) = hi;
+                if (tail && key0 + rr >= k1) vr[i] = u32x4{0, 0, 0, 0}, vsr[i] = 127;
+                e4m3_expand<T>(vr[i], e4m3_scale(vsr[i]), lo, hi);
+                *(v8*)(my_v + rr * VSTR + 16 * lcol) = lo;
+                *(v8*)(my_v + rr * VSTR + 16 * lcol + 8) = hi;
+            } else {
+                *(u32x4*)(my_k + rr * KSTR + 8 * lcol) = kr[i];
+                if (tail && key0 + rr >= k1) vr[i] = u32x4{0, 0, 0, 0};
+                *(u32x4*)(my_v + rr * VSTR + 8 * lcol) = vr[i];
+            }
+        }
+        const int nxt = key0 + PAD_NW * PAD_BK;
+        if (nxt < k1) {
+            load(nxt, pa, pb);
+            if (nxt + PAD_NW * PAD_BK < k1) pages(nxt + PAD_NW * PAD_BK, pa, pb);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        floatx4 s_acc[MT][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            v8 kf[DSTEPS];
+#pragma unroll
+            for (int s = 0; s < DSTEPS; ++s) kf[s] = *(const v8*)(my_k + (16 * t + qc) * KSTR + 32 * s + 8 * g);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < DSTEPS; ++s) acc = mfma16<T>(kf[s], qf[mt][s], acc);
+                s_acc[mt][t] = acc;
+            }
+        }
+        const bool masked = tail || key0 + PAD_BK - 1 > lim0;
+        v8 pf[MT];
+        float alpha[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float sv[8], cmax = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float x = s_acc[mt][j >> 2][j & 3] * P.scale_log2e;
+                if (masked) {
+                    const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                    x = key < k1 && key <= lim[mt] ? x : -INFINITY;
+                }
+                sv[j] = x;
+                cmax = fmaxf(cmax, x);
+            }
+            cmax = group4_max(cmax);
+            const float m_new = fmaxf(m_run[mt], cmax);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;       // nothing seen so far
+            alpha[mt] = __builtin_amdgcn_exp2f(m_run[mt] - m_use);
+            float psum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float p = __builtin_amdgcn_exp2f(sv[j] - m_use);
+                psum += p;
+                pf[mt][j] = (T)p;
+            }
+            l_run[mt] = l_run[mt] * alpha[mt] + psum;
+            m_run[mt] = m_new;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const T* a0 = my_v + (4 * g + (qc >> 2)) * VSTR + 16 * nt + 4 * (qc & 3);
+            const u32x2 lo = read_transposed(a0), hi = read_transposed(a0 + 16 * VSTR);
+            const v8 vf = __builtin_bit_cast(v8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                floatx4 o = o_acc[mt][nt];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[r] *= alpha[mt];
+                if (!masked) {
+                    o_acc[mt][nt] = mfma16<T>(vf, pf[mt], o);
+                    continue;
+                }
+                // some row of the tile does not see some key here: a weight of 0 must not meet an infinity or a NaN
+                const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+                floatx4 add = mfma16<T>(vf, pf[mt], zero);
+                if (__any(!(__builtin_fabsf((add[0] + add[1]) + (add[2] + add[3])) < INFINITY))) {
+                    add = mfma16<T>(finite_part(vf), pf[mt], zero);
+                    v8 seen;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                        seen[j] = key < k1 && key <= lim[mt] ? 1 : 0;
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < 3; ++c) {
+                        const floatx4 n = mfma16<T>(class_part(vf, c), seen, zero);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) add[r] += n[r] > 0.f ? (c == 0 ? INFINITY : c == 1 ? -INFINITY : NAN) : 0.f;
+                    }
+                }
+                o_acc[mt][nt] = o + add;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // ---- join the waves -------------------------------------------------------------------------
+    __syncthreads();                                // everyone is done with the staging area
+    float* lds_o = (float*)lds;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const float l = group4_sum(l_run[mt]);
+        if (g == 0) { lds_ml[wave][16 * mt + qc][0] = m_run[mt]; lds_ml[wave][16 * mt + qc][1] = l; }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) *(floatx4*)(lds_o + (wave * ROWS + 16 * mt + qc) * OSTR + 16 * nt + 4 * g) = o_acc[mt][nt];
+    }
+    __syncthreads();
+    for (int e = tid; e < ROWS * (D / 4); e += PAD_NW * 64) {
+        const int row = e / (D / 4), col = 4 * (e % (D / 4)), r = I.row0 + row;
+        if (r >= I.rows) break;                     // rows ascend with e
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < PAD_NW; ++w) m = fmaxf(m, lds_ml[w][row][0]);
+        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < PAD_NW; ++w) {
+            const float mw = lds_ml[w][row][0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
+            l += lds_ml[w][row][1] * f;
+            o += *(const floatx4*)(lds_o + (w * ROWS + row) * OSTR + col) * f;
+        }
+        const int token = r / P.group, head = I.kvh * P.group + r - token * P.group;
+        if (I.n_parts <= 1) {
+            const float inv = l != 0.f ? 1.0f / l : 0.f;            // a row that sees nothing: zeros
+            v4 res;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) res[j] = (T)(o[j] * inv);
+            *(v4*)((T*)P.out + (size_t)(I.first + token) * P.out_stride + (size_t)head * D + col) = res;
+        } else {
+            const size_t pr = ((size_t)I.split * P.n_rows + I.first + token) * P.n_heads + head;
+            *(floatx4*)(P.part_o + pr * D + col) = o;
+            if (col == 0) { P.part_ml[pr * 2] = m; P.part_ml[pr * 2 + 1] = l; }
+        }
+    }
+}
+
+// Joins the parts of the key axis: one workgroup a (row, head), its waves take the parts in turn.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_attention_join_kernel(PagedAttnParams P, int tile_rows) {
+    __shared__ float acc[4][D];
+    const int t = blockIdx.x / P.n_heads, head = blockIdx.x % P.n_heads, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int seq = seq_of_row(P.cu_rows, P.n_seqs, t);
+    if (seq >= P.n_seqs) return;
+    const int first = P.cu_rows[seq], rows = (P.cu_rows[seq + 1] - first) * P.group, past = P.seq_lens[seq];
+    const int r = (t - first) * P.group + head % P.group;
+    const int parts = (attn_tile_end(P, past, rows, r / tile_rows, tile_rows) + P.split_len - 1) / P.split_len;
+    if (parts <= 1) return;                         // written already
+    const size_t step = (size_t)P.n_rows * P.n_heads, row = (size_t)t * P.n_heads + head;
+    const bool mine = lane < parts;                 // at most 64 parts
+    const float m = mine ? P.part_ml[(row + lane * step) * 2] : -INFINITY, l = mine ? P.part_ml[(row + lane * step) * 2 + 1] : 0.f;
+    const float top = wave_max_f32_dpp(m);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float sum = wave_sum_f32_dpp(l * f);
+    constexpr int E = D / 64;
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int s = wave; s < parts; s += 4) {
+        const float fs = __shfl(f, s, 64);
+        const float* src = P.part_o + (row + s * step) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += src[e] * fs;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[wave][lane * E + e] = o[e];
+    __syncthreads();
+    for (int d = threadIdx.x; d < D; d += 256) {
+        const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+        ((T*)P.out)[(size_t)t * P.out_stride + (size_t)head * D + d] = (T)(((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv);
+    }
+}
+
+struct AttnPlan { int tile_rows, n_tiles, n_splits, split_len; };
+
+static AttnPlan attn_plan(int n_seqs, int max_rows, int max_len, int n_heads, int h_kv) {
+    AttnPlan A;
+    const int rows = max_rows * (n_heads / h_kv);
+    A.tile_rows = rows <= 16 ? 16 : 32;
+    A.n_tiles = (rows + A.tile_rows - 1) / A.tile_rows;
+    const int64_t base = (int64_t)n_seqs * h_kv * A.n_tiles;
+    int64_t want = (2048 + base - 1) / base;
+    want = want > 64 ? 64 : want;
+    int64_t len = (max_len + want - 1) / want;
+    len = len < 256 ? 256 : len;
+    A.split_len = (int)((len + 127) / 128 * 128);
+    A.n_splits = (max_len + A.split_len - 1) / A.split_len;
+    if (A.n_splits < 1) A.n_splits = 1;
+    return A;
+}
+
+extern "C" size_t sq_paged_attention_workspace_bytes(int n_seqs, int n_rows, int max_rows, int max_len, int n_heads, int h_kv, int d) {
+    if (n_seqs <= 0 || n_rows <= 0 || max_rows <= 0 || max_len <= 0 || n_heads <= 0 || h_kv <= 0 || n_heads % h_kv || d <= 0) return 0;
+    if (max_rows > n_rows) max_rows = n_rows;
+    const AttnPlan A = attn_plan(n_seqs, max_rows, max_len, n_heads, h_kv);
+    return A.n_splits > 1 ? (size_t)A.n_splits * n_rows * n_heads * (d + 2) * sizeof(float) : 0;
+}
+
+extern "C" int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t q_row_stride, const void* k_pages, const void* v_pages,
+                                  const void* k_scales, const void* v_scales, void* out, int64_t out_stride,
+                                  const int32_t* d_page_table, int table_width, int n_pages, int page_size, const int32_t* d_seq_lens,
+                                  const int32_t* d_cu_rows, int n_seqs, int n_rows, int max_rows, int max_len, int n_heads, int h_kv,
+                                  int d, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (n_seqs < 0 || n_rows < 0 || max_rows < 0 || max_len < 0 || n_heads <= 0 || h_kv <= 0 || n_heads % h_kv || table_width < 0 || n_pages <= 0)
+        return SQ_EINVAL;
+    if (!k_scales != !v_scales || !(scale > 0.f) || !(scale < INFINITY)) return SQ_EINVAL;
+    const int shift = page_shift(page_size);
+    if ((d != 64 && d != 128) || shift < 0 || (dtype != SQ_DTYPE_F16 && dtype != SQ_DTYPE_BF16)) return SQ_EUNSUPPORTED;
+    if (n_rows == 0 || n_seqs == 0 || max_rows == 0) return SQ_OK;
+    if (max_len < 1 || (int64_t)max_len > ((int64_t)table_width << shift)) return SQ_EINVAL;
+    if (!q || !k_pages || !v_pages || !out || !d_page_table || !d_seq_lens || !d_cu_rows) return SQ_EINVAL;
+    if ((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) || ((uintptr_t)out & 7) || ((q_head_stride | q_row_stride) & 7) || (out_stride & 3))
+        return SQ_EINVAL;
+    if (max_rows > n_rows) max_rows = n_rows;
+    const AttnPlan A = attn_plan(n_seqs, max_rows, max_len, n_heads, h_kv);
+    const size_t need = sq_paged_attention_workspace_bytes(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d);
+    if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return SQ_EINVAL;
+    const int64_t grid = (int64_t)n_seqs * h_kv * A.n_tiles * A.n_splits, join = (int64_t)n_rows * n_heads;
+    if (grid > 0x7fffffff || join > 0x7fffffff) return SQ_EUNSUPPORTED;
+    PagedAttnParams P = {q, q_head_stride, q_row_stride, k_pages, v_pages, (const uint8_t*)k_scales, (const uint8_t*)v_scales, out, out_stride,
+                         {d_page_table, table_width, n_pages, shift}, d_seq_lens, d_cu_rows, n_seqs, n_rows, n_heads, h_kv, n_heads / h_kv,
+                         scale * 1.4426950408889634f, max_len, A.n_tiles, A.n_splits, A.split_len, (float*)workspace,
+                         need ? (float*)workspace + (size_t)A.n_splits * n_rows * n_heads * d : nullptr};
+    hipStream_t st = (hipStream_t)stream;
+#define SQ_A(TT, DD, QQ, MM) hipLaunchKernelGGL((paged_attention_rows_kernel<TT, DD, QQ, MM>), dim3((unsigned)grid), dim3(PAD_NW * 64), 0, st, P)
+#define SQ_AM(TT, DD, QQ) do { if (A.tile_rows == 16) SQ_A(TT, DD, QQ, 1); else SQ_A(TT, DD, QQ, 2); } while (0)
+#define SQ_AD(TT, DD) do { if (k_scales) SQ_AM(TT, DD, true); else SQ_AM(TT, DD, false); } while (0)
+    if (dtype == SQ_DTYPE_F16) { if (d == 128) SQ_AD(half_t, 128); else SQ_AD(half_t, 64); }
+    else                       { if (d == 128) SQ_AD(bf16_t, 128); else SQ_AD(bf16_t, 64); }
+#undef SQ_AD
+#undef SQ_AM
+#undef SQ_A
+    int rc = sq_check_launch();
+    if (rc != SQ_OK || A.n_splits <= 1) return rc;
+#define SQ_J(TT, DD) hipLaunchKernelGGL((paged_attention_join_kernel<TT, DD>), dim3((unsigned)join), dim3(256), 0, st, P, A.tile_rows)
+    if (dtype == SQ_DTYPE_F16) { if (d == 128) SQ_J(half_t, 128); else SQ_J(half_t, 64); }
+    else                       { if (d == 128) SQ_J(bf16_t, 128); else SQ_J(bf16_t, 64); }
+#undef SQ_J
+    return sq_check_launch();
+}

@@ -47,33 +47,6 @@ struct AttnParams {
     int xcd_span;           // h_kv < 8: XCDs one KV head's workgroups are dealt over (host: att_xcd_span)
 };
 
-// max / sum over the four 16-lane groups holding the same query (lanes l, l^16, l^32, l^48) with the
-// gfx950 VALU lane swaps (v_permlane16_swap / v_permlane32_swap) instead of LDS-routed ds_bpermute
-// (inline asm: with ROCm 7.2's clang the __builtin_amdgcn_permlane*_swap builtins return the first
-// result twice; the s_nop's are the VALU-write -> permlane-read wait states hipcc would insert.)
-__device__ __forceinline__ void lane_swap16(unsigned& a, unsigned& b) {
-    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
-}
-__device__ __forceinline__ void lane_swap32(unsigned& a, unsigned& b) {
-    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
-}
-__device__ __forceinline__ float group4_max(float v) {
-    unsigned a = __builtin_bit_cast(unsigned, v), b = a;
-    lane_swap16(a, b);                   // a = rows [0,0,2,2], b = rows [1,1,3,3]
-    v = fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
-    a = __builtin_bit_cast(unsigned, v); b = a;
-    lane_swap32(a, b);                   // a = lower half twice, b = upper half twice
-    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
-}
-__device__ __forceinline__ float group4_sum(float v) {
-    unsigned a = __builtin_bit_cast(unsigned, v), b = a;
-    lane_swap16(a, b);
-    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
-    a = __builtin_bit_cast(unsigned, v); b = a;
-    lane_swap32(a, b);
-    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
-}
-
 // MASK: 0 = dense additive mask, 1 = tree mask with the bitmask row in two registers (n <= 128),
 // 2 = tree mask with the bitmask rows staged in LDS (n <= 512).
 // (A variant that also applied RoPE and wrote the new K/V rows -- one launch instead of sq_rope_kv_write_f16 + this

@@ -13,6 +13,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SEQUOIA_LIB") or os.path.join(_PKG, "lib", "libsequoia_hip.so")
 
 SQ_OK, SQ_EINVAL, SQ_EUNSUPPORTED, SQ_ELAUNCH = 0, -1, -2, -3
+SQ_DTYPE_F16, SQ_DTYPE_BF16, SQ_DTYPE_F32 = 0, 1, 2
 SQ_MAX_TREE = 512
 SQ_MAX_TOPK = 128
 SQ_RESULT_INTS = 64
@@ -77,6 +78,14 @@ PROTOTYPES = {
                                      _vp, _i, _vp, _i, _vp]),
     "sq_level_attention_f16": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _i, _vp, _i,
                                     _vp, _vp]),
+    "sq_rope_kv_write_paged": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _i,
+                                    _i, _vp]),
+    "sq_kv_read_paged": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "sq_paged_attention_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i, _i]),
+    "sq_paged_attention": (_i, [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f,
+                                _i, _vp, C.c_size_t, _vp]),
+    "sq_verify_drafts_workspace_bytes": (C.c_size_t, [_i, _i, _i]),
+    "sq_verify_drafts": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _f, _vp, _vp, _i, _vp, C.c_size_t, _vp]),
     "sq_ar_workspace_bytes": (C.c_size_t, [_i, C.c_size_t, C.c_size_t]),
     "sq_ar_alloc": (_i, [C.POINTER(_vp), C.c_size_t]),
     "sq_ar_free": (_i, [_vp]),

@@ -32,6 +32,50 @@ def _need(t: torch.Tensor, dtype, name: str, contiguous: bool = True):
     return t
 
 
+_DTYPE_CODES = {torch.float16: native.SQ_DTYPE_F16, torch.bfloat16: native.SQ_DTYPE_BF16, torch.float32: native.SQ_DTYPE_F32}
+
+
+def _on_device(dev, **tensors):
+    """Every tensor on the device `dev` of the call (None is allowed): the launch goes to that device's current stream."""
+    if dev.type != "cuda":
+        raise native.SequoiaNativeError(f"the tensors live on {dev}: the paged path only runs on a HIP device (no CPU fallback)")
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: lives on {t.device}, the call's tensors on {dev}")
+
+
+def _index(t, dtype, n, name):
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.dim() != 1 or not t.is_contiguous() or t.shape[0] < n:
+        raise ValueError(f"{name}: expected {n} contiguous entries, got {tuple(t.shape)}")
+
+
+def _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dtype):
+    """Checks the pages of one layer; -> (n_pages, H_kv, page_size, D, sequences, table width)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
+        raise ValueError(f"k_pages / v_pages: expected [n_pages, H_kv, page_size, D] twice, got {tuple(shape)}, {tuple(v_pages.shape)}")
+    want = dtype if k_scales is None else torch.float8_e4m3fn
+    if k_pages.dtype != want or v_pages.dtype != want:
+        raise TypeError(f"k_pages / v_pages: expected {want}, got {k_pages.dtype}, {v_pages.dtype}")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("k_pages / v_pages: must be contiguous")
+    if (k_scales is None) != (v_scales is None):
+        raise ValueError("k_scales / v_scales: both or none")
+    if k_scales is not None:
+        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            if t.dtype != torch.uint8:
+                raise TypeError(f"{name}: expected torch.uint8, got {t.dtype}")
+            if t.shape != shape[:3] or not t.is_contiguous():
+                raise ValueError(f"{name}: expected {tuple(shape[:3])} contiguous, got {tuple(t.shape)}")
+    if page_table.dtype != torch.int32:
+        raise TypeError(f"page_table: expected torch.int32, got {page_table.dtype}")
+    if page_table.dim() != 2 or not page_table.is_contiguous():
+        raise ValueError(f"page_table: expected [sequences, pages] contiguous, got {tuple(page_table.shape)}")
+    return (*shape, *page_table.shape)
+
+
 class HipOps:
     name = "hip"
 
@@ -375,6 +419,152 @@ class HipOps:
                                             _ptr(child_ids), n_tree, vocab, int(gt), workspace.data_ptr(), result.data_ptr(),
                                             _ptr(step), _ptr(result_ring), self._stream()), "sq_verify_greedy_f16")
         return result
+
+    # ---- batched speculative decoding over a paged KV cache -------------------------------------
+    def _launch(self, dev, fn, what, args):
+        """fn(*args, stream) on `dev`'s current stream, with `dev` current for the launch."""
+        if dev.index == torch.cuda.current_device():
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        if rc:
+            check(rc, what)
+
+    def rope_kv_write_paged(self, qkv, q_out, k_pages, v_pages, cos, sin, position_ids, page_table, seq_lens, cu_rows, n_heads, h_kv,
+                            d, k_scales=None, v_scales=None):
+        """RoPE of the packed rows qkv [n_rows, (H + 2 H_kv) D] of a ragged batch into q_out [H, n_rows, D], and the write of K and
+        V behind each sequence's stored rows: row cu_rows[b] + i goes to row seq_lens[b] + i of sequence b.  Pages
+        [n_pages, H_kv, page_size, D] in qkv's type, or float8_e4m3fn with k_scales / v_scales (uint8, [n_pages, H_kv, page_size]).
+        Rows behind cu_rows[-1] are left alone."""
+        dev, dt = qkv.device, qkv.dtype
+        _on_device(dev, q_out=q_out, k_pages=k_pages, v_pages=v_pages, cos=cos, sin=sin, position_ids=position_ids, page_table=page_table,
+                   seq_lens=seq_lens, cu_rows=cu_rows, k_scales=k_scales, v_scales=v_scales)
+        if dt not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"qkv: expected torch.float16 or torch.bfloat16, got {dt}")
+        for t, name in ((q_out, "q_out"), (cos, "cos"), (sin, "sin")):
+            if t.dtype != dt:
+                raise TypeError(f"{name}: expected {dt}, got {t.dtype}")
+        n_pages, hk, page_size, dim, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
+        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (n_heads + 2 * h_kv) * d or (hk, dim) != (h_kv, d):
+            raise ValueError(f"qkv: expected [n_rows, {(n_heads + 2 * h_kv) * d}] with unit inner stride over pages of {h_kv} heads of {d}, "
+                             f"got {tuple(qkv.shape)} over {hk} heads of {dim}")
+        n_rows = qkv.shape[0]
+        if q_out.shape != (n_heads, n_rows, d) or not q_out.is_contiguous():
+            raise ValueError(f"q_out: expected {(n_heads, n_rows, d)} contiguous, got {tuple(q_out.shape)}")
+        if cos.dim() != 2 or cos.shape[1] != d or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError(f"cos / sin: expected [positions, {d}] contiguous twice, got {tuple(cos.shape)}, {tuple(sin.shape)}")
+        _index(position_ids, torch.int64, n_rows, "position_ids")
+        _index(seq_lens, torch.int32, n_seqs, "seq_lens")
+        _index(cu_rows, torch.int32, n_seqs + 1, "cu_rows")
+        self._launch(dev, self.lib.sq_rope_kv_write_paged, "sq_rope_kv_write_paged",
+                     (qkv.data_ptr(), qkv.stride(0) if n_rows > 1 else qkv.shape[1], q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                      _ptr(k_scales), _ptr(v_scales), cos.data_ptr(), sin.data_ptr(), cos.shape[0], position_ids.data_ptr(),
+                      page_table.data_ptr(), width, n_pages, page_size, seq_lens.data_ptr(), cu_rows.data_ptr(), n_seqs, n_rows, n_heads,
+                      h_kv, d, _DTYPE_CODES[dt]))
+
+    def kv_read_paged(self, k_pages, v_pages, k_out, v_out, page_table, starts, counts, max_count=None, k_scales=None, v_scales=None):
+        """Stored rows [starts[b], starts[b] + counts[b]) of every sequence into rows [0, counts[b]) of k_out / v_out
+        [sequences, H_kv, M, D] (fp16 or bf16, rows contiguous: layer slabs of static caches fit).  Other rows stay as they are.
+        max_count: no sequence asks for more rows (default: M); rows beyond it are not read."""
+        dev, dt = k_out.device, k_out.dtype
+        _on_device(dev, k_pages=k_pages, v_pages=v_pages, v_out=v_out, page_table=page_table, starts=starts, counts=counts,
+                   k_scales=k_scales, v_scales=v_scales)
+        if dt not in (torch.float16, torch.bfloat16) or v_out.dtype != dt:
+            raise TypeError(f"k_out / v_out: expected torch.float16 or torch.bfloat16 twice, got {dt}, {v_out.dtype}")
+        n_pages, h_kv, page_size, d, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
+        if k_out.dim() != 4 or (k_out.shape[0], k_out.shape[1], k_out.shape[3]) != (n_seqs, h_kv, d) or v_out.shape != k_out.shape:
+            raise ValueError(f"k_out / v_out: expected [{n_seqs}, {h_kv}, M, {d}] twice, got {tuple(k_out.shape)}, {tuple(v_out.shape)}")
+        m = k_out.shape[2]
+        s = k_out.stride()
+        if v_out.stride() != s or s[3] != 1 or (m > 1 and s[2] != d) or (h_kv > 1 and s[1] < m * d) or (n_seqs > 1 and s[0] < m * d):
+            raise ValueError(f"k_out / v_out: expected contiguous rows and the same strides, got {s}, {v_out.stride()}")
+        _index(starts, torch.int32, n_seqs, "starts")
+        _index(counts, torch.int32, n_seqs, "counts")
+        if max_count is None:
+            max_count = m
+        if not 0 <= max_count <= m:
+            raise ValueError(f"max_count: {max_count} is not between 0 and {m}")
+        self._launch(dev, self.lib.sq_kv_read_paged, "sq_kv_read_paged",
+                     (k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), k_out.data_ptr(), v_out.data_ptr(),
+                      s[0] if n_seqs > 1 else h_kv * m * d, s[1] if h_kv > 1 else m * d, m, page_table.data_ptr(), width, n_pages, page_size,
+                      starts.data_ptr(), counts.data_ptr(), n_seqs, int(max_count), h_kv, d, _DTYPE_CODES[dt]))
+        return k_out, v_out
+
+    def paged_attention(self, q, k_pages, v_pages, out, page_table, seq_lens, cu_rows, scale, max_rows=None, max_len=None, k_scales=None,
+                        v_scales=None):
+        """Attention of a ragged batch's new tokens (written before by rope_kv_write_paged): row cu_rows[b] + i of q [H, n_rows, D]
+        sees keys [0, seq_lens[b] + i] of sequence b; out [n_rows, H D].  max_rows / max_len: no sequence brings more rows / ends
+        behind more keys (defaults: n_rows, the table's whole width); they size the launch, and rows and keys beyond them are left
+        out.  The default max_len costs workgroups that find nothing to do."""
+        dev, dt = q.device, q.dtype
+        _on_device(dev, k_pages=k_pages, v_pages=v_pages, out=out, page_table=page_table, seq_lens=seq_lens, cu_rows=cu_rows,
+                   k_scales=k_scales, v_scales=v_scales)
+        if dt not in (torch.float16, torch.bfloat16) or out.dtype != dt:
+            raise TypeError(f"q / out: expected torch.float16 or torch.bfloat16 twice, got {dt}, {out.dtype}")
+        n_pages, h_kv, page_size, d, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
+        if q.dim() != 3 or q.shape[2] != d or q.shape[0] % h_kv or q.stride(2) != 1:
+            raise ValueError(f"q: expected [H, n_rows, {d}] with unit inner stride and a multiple of {h_kv} heads, got {tuple(q.shape)}")
+        n_heads, n_rows = q.shape[0], q.shape[1]
+        if out.shape != (n_rows, n_heads * d) or out.stride(1) != 1 or (n_rows > 1 and out.stride(0) < n_heads * d):
+            raise ValueError(f"out: expected {(n_rows, n_heads * d)} with unit inner stride, got {tuple(out.shape)}")
+        _index(seq_lens, torch.int32, n_seqs, "seq_lens")
+        _index(cu_rows, torch.int32, n_seqs + 1, "cu_rows")
+        max_rows = n_rows if max_rows is None else min(int(max_rows), n_rows)
+        max_len = width * page_size if max_len is None else int(max_len)
+        if max_rows < 0 or not 0 <= max_len <= width * page_size:
+            raise ValueError(f"max_rows {max_rows} / max_len {max_len}: the table holds {width * page_size} keys a sequence")
+        if not 0.0 < scale < float("inf"):
+            raise ValueError(f"scale: expected a positive number, got {scale}")
+        need = self.lib.sq_paged_attention_workspace_bytes(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d)
+        # one buffer a call, from the stream-ordered allocator: two streams or two captured graphs never share it
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        self._launch(dev, self.lib.sq_paged_attention, "sq_paged_attention",
+                     (q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+                      out.data_ptr(), out.stride(0) if n_rows > 1 else n_heads * d, page_table.data_ptr(), width, n_pages, page_size,
+                      seq_lens.data_ptr(), cu_rows.data_ptr(), n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d, float(scale),
+                      _DTYPE_CODES[dt], _ptr(ws), need))
+        return out
+
+    def verify_drafts(self, target_logits, draft_logits, draft_tokens, cu_drafts, u_accept, u_next, temperature, n_accepted, next_tokens):
+        """Verifies a batch's drafted tokens from given uniforms in [0, 1).  Sequence b drafted draft_tokens[cu_drafts[b] :
+        cu_drafts[b + 1]]; target_logits [>= drafts + sequences, V] row cu_drafts[b] + b + i judges its token i and the row behind its
+        last one follows, draft_logits [>= drafts, V] are the rows the tokens were drawn from.  Tokens are accepted while
+        u_accept q(token) < p(token); then the next token is drawn with u_next[b] from max(p - q, 0), or from p behind the last one.
+        temperature: a number or a float32 tensor [sequences]; 0 is greedy.  n_accepted int32 / next_tokens int64 [sequences]
+        (-1: the deciding row is no distribution)."""
+        dev, dt = target_logits.device, target_logits.dtype
+        temps = temperature if isinstance(temperature, torch.Tensor) else None
+        _on_device(dev, draft_logits=draft_logits, draft_tokens=draft_tokens, cu_drafts=cu_drafts, u_accept=u_accept, u_next=u_next,
+                   temperature=temps, n_accepted=n_accepted, next_tokens=next_tokens)
+        if dt not in _DTYPE_CODES or draft_logits.dtype != dt:
+            raise TypeError(f"target_logits / draft_logits: expected fp16, bf16 or fp32 twice, got {dt}, {draft_logits.dtype}")
+        n_seqs, n_drafts = n_accepted.shape[0], draft_tokens.shape[0]
+        if target_logits.dim() != 2 or draft_logits.dim() != 2 or target_logits.shape[1] != draft_logits.shape[1]:
+            raise ValueError(f"target_logits / draft_logits: expected two dimensions and one vocabulary, got {tuple(target_logits.shape)}, "
+                             f"{tuple(draft_logits.shape)}")
+        vocab = target_logits.shape[1]
+        for t, rows, name in ((target_logits, n_drafts + n_seqs, "target_logits"), (draft_logits, n_drafts, "draft_logits")):
+            if t.shape[0] < rows or (rows and t.stride(1) != 1) or (rows > 1 and t.stride(0) < vocab):
+                raise ValueError(f"{name}: expected {rows} rows with unit inner stride, got {tuple(t.shape)}")
+        _index(draft_tokens, torch.int64, n_drafts, "draft_tokens")
+        _index(cu_drafts, torch.int32, n_seqs + 1, "cu_drafts")
+        _index(u_accept, torch.float32, n_drafts, "u_accept")
+        _index(u_next, torch.float32, n_seqs, "u_next")
+        _index(n_accepted, torch.int32, n_seqs, "n_accepted")
+        _index(next_tokens, torch.int64, n_seqs, "next_tokens")
+        if temps is not None:
+            _index(temps, torch.float32, n_seqs, "temperature")
+        elif not 0.0 <= temperature < float("inf"):
+            raise ValueError(f"temperature: expected a number >= 0, got {temperature}")
+        need = self.lib.sq_verify_drafts_workspace_bytes(n_seqs, n_drafts, vocab)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        self._launch(dev, self.lib.sq_verify_drafts, "sq_verify_drafts",
+                     (target_logits.data_ptr(), max(target_logits.stride(0), vocab), _ptr(draft_logits) or None,
+                      max(draft_logits.stride(0), vocab), _ptr(draft_tokens) or None, cu_drafts.data_ptr(), n_seqs, n_drafts, vocab,
+                      _ptr(u_accept) or None, u_next.data_ptr(), _ptr(temps), 0.0 if temps is not None else float(temperature),
+                      n_accepted.data_ptr(), next_tokens.data_ptr(), _DTYPE_CODES[dt], ws.data_ptr(), need))
+        return n_accepted, next_tokens
 
     # ---- row-wise glue ------------------------------------------------------------------------
     def rmsnorm(self, x, weight, out, eps):
