@@ -6,6 +6,7 @@
 // head r % group), so that every stored row is read once for all of them.
 #include "paged.h"
 #include "attn_map.h"
+#include <type_traits>
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef __fp16 fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
@@ -30,24 +31,43 @@ template <typename T> __device__ __forceinline__ floatx4 mfma16(typename vec_of<
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+template <typename T> __device__ __forceinline__ floatx16 mfma32(typename vec_of<T>::v8 a, typename vec_of<T>::v8 b, floatx16 c) {
+    if constexpr (__is_same(T, half_t)) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
 // column (lane & 15) of the 4 x 16 block of 16-bit values whose row (lane & 15) >> 2, columns 4 (lane & 3).. this lane addresses
 __device__ __forceinline__ u32x2 read_transposed(const void* p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)p));
 }
 
-// elements of v that are not finite, as 0; of class c (0: +inf, 1: -inf, 2: NaN), as 1 and the others as 0
-template <typename V8> __device__ __forceinline__ V8 finite_part(V8 v) {
+// A weight of 0 must not meet an infinity or a NaN in a row of V that some query does not see.  Where a chunk of keys holds such
+// rows, what is not finite is staged as 0 and its rows are noted; add_hidden puts it back for the queries that do see it.
+// Returns whether anything of v was not finite (an exponent of all ones: adding one to it carries into the sign's place).
+template <typename T> __device__ __forceinline__ bool take_nonfinite(typename vec_of<T>::v8& v) {
+    constexpr uint32_t E = __is_same(T, half_t) ? 0x7c007c00u : 0x7f807f80u, ONE = __is_same(T, half_t) ? 0x04000400u : 0x00800080u;
+    u32x4 w = __builtin_bit_cast(u32x4, v);
+    uint32_t any = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __builtin_fabsf((float)v[j]) < INFINITY ? v[j] : 0;
-    return v;
-}
-template <typename V8> __device__ __forceinline__ V8 class_part(V8 v, int c) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float x = (float)v[j];
-        v[j] = (c == 0 ? x == INFINITY : c == 1 ? x == -INFINITY : x != x) ? 1 : 0;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t bad = ((w[i] & E) + ONE) & 0x80008000u;
+        any |= bad;
+        w[i] &= ~(bad | (bad - (bad >> 15)));
     }
-    return v;
+    v = __builtin_bit_cast(typename vec_of<T>::v8, w);
+    return any != 0;
+}
+// the four elements of a stored row of V from column d on, those that are finite as 0
+template <typename T, int D, bool Q8> __device__ __forceinline__ void hidden4(const PagedAttnParams& P, size_t row, int d, float (&x)[4]) {
+    if constexpr (Q8) {
+        const uint32_t w = *(const uint32_t*)((const uint8_t*)P.v + row * D + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = ((w >> (8 * j)) & 0x7fu) == 0x7fu ? NAN : 0.f;
+    } else {
+        const typename vec_of<T>::v4 w = *(const typename vec_of<T>::v4*)((const T*)P.v + row * D + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __builtin_fabsf((float)w[j]) < INFINITY ? 0.f : (float)w[j];
+    }
 }
 
 // what a workgroup works on
@@ -76,6 +96,10 @@ __device__ __forceinline__ bool attn_item(const PagedAttnParams& P, int tile_row
     I.end = attn_tile_end(P, I.past, I.rows, tile, tile_rows);
     I.n_parts = (I.end + P.split_len - 1) / P.split_len;
     return I.split < I.n_parts || (I.split == 0 && I.n_parts == 0);
+}
+
+__device__ __forceinline__ size_t stored_row(const PagedAttnParams& P, int page, int kvh, int key) {
+    return (((size_t)page * P.h_kv + kvh) << P.map.shift) + (key & ((1 << P.map.shift) - 1));
 }
 
 // Few rows (a decoding step, a drafted chunk): bound by the bytes of K and V.  Four waves walk the 32-key chunks of the
@@ -139,7 +163,7 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int rr = i * RPP + lrow;
-            const size_t r = (((size_t)(i * RPP < 16 ? pa : pb) * P.h_kv + I.kvh) << P.map.shift) + ((key0 + rr) & ((1 << P.map.shift) - 1));
+            const size_t r = stored_row(P, i * RPP < 16 ? pa : pb, I.kvh, key0 + rr);
             const size_t at = r * D * (Q8 ? 1 : 2) + 16 * lcol;
             kr[i] = *(const u32x4*)((const uint8_t*)P.k + at);
             vr[i] = *(const u32x4*)((const uint8_t*)P.v + at);
@@ -154,22 +178,33 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
     }
     for (; key0 < k1; key0 += PAD_NW * PAD_BK) {
         const bool tail = key0 + PAD_BK > k1;       // rows behind the end hold anything: their weights are 0, and so are they
+        const bool masked = tail || key0 + PAD_BK - 1 > lim0;
+        uint32_t hidden = 0;                        // rows of the chunk with values that were taken out
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int rr = i * RPP + lrow;
+            bool bad = false;
             if constexpr (Q8) {
                 v8 lo, hi;
                 e4m3_expand<T>(kr[i], e4m3_scale(ksr[i]), lo, hi);
                 *(v8*)(my_k + rr * KSTR + 16 * lcol) = lo;
                 *(v8*)(my_k + rr * KSTR + 16 * lcol + 8) = hi;
-                if (tail && key0 + rr >= k1) vr[i] = u32x4{0, 0, 0, 0}, vsr[i] = 127;
+                if (tail && key0 + rr >= k1) { vr[i] = u32x4{0, 0, 0, 0}; vsr[i] = 127; }
                 e4m3_expand<T>(vr[i], e4m3_scale(vsr[i]), lo, hi);
+                if (masked) bad = take_nonfinite<T>(lo) | take_nonfinite<T>(hi);
                 *(v8*)(my_v + rr * VSTR + 16 * lcol) = lo;
                 *(v8*)(my_v + rr * VSTR + 16 * lcol + 8) = hi;
             } else {
                 *(u32x4*)(my_k + rr * KSTR + 8 * lcol) = kr[i];
                 if (tail && key0 + rr >= k1) vr[i] = u32x4{0, 0, 0, 0};
-                *(u32x4*)(my_v + rr * VSTR + 8 * lcol) = vr[i];
+                v8 w = __builtin_bit_cast(v8, vr[i]);
+                if (masked) bad = take_nonfinite<T>(w);
+                *(v8*)(my_v + rr * VSTR + 8 * lcol) = w;
+            }
+            if (masked) {
+                const uint64_t lanes = __ballot(bad);
+                if (lanes)
+                    for (int j = 0; j < RPP; ++j) hidden |= (uint32_t)(((lanes >> (j * LPR)) & ((1ull << LPR) - 1)) != 0) << (i * RPP + j);
             }
         }
         const int nxt = key0 + PAD_NW * PAD_BK;
@@ -193,7 +228,6 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
                 s_acc[mt][t] = acc;
             }
         }
-        const bool masked = tail || key0 + PAD_BK - 1 > lim0;
         v8 pf[MT];
         float alpha[MT];
 #pragma unroll
@@ -235,29 +269,21 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
                 floatx4 o = o_acc[mt][nt];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] *= alpha[mt];
-                if (!masked) {
-                    o_acc[mt][nt] = mfma16<T>(vf, pf[mt], o);
-                    continue;
-                }
-                // some row of the tile does not see some key here: a weight of 0 must not meet an infinity or a NaN
-                const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
-                floatx4 add = mfma16<T>(vf, pf[mt], zero);
-                if (__any(!(__builtin_fabsf((add[0] + add[1]) + (add[2] + add[3])) < INFINITY))) {
-                    add = mfma16<T>(finite_part(vf), pf[mt], zero);
-                    v8 seen;
+                o_acc[mt][nt] = mfma16<T>(vf, pf[mt], o);
+            }
+        }
+        while (hidden) {                            // wave-uniform, and hardly ever entered
+            const int key = key0 + __builtin_ctz(hidden), page = page_of(P.map, I.seq, key >> P.map.shift);
+            hidden &= hidden - 1;
+            const size_t row = stored_row(P, page < 0 ? 0 : page, I.kvh, key);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                        seen[j] = key < k1 && key <= lim[mt] ? 1 : 0;
-                    }
-#pragma unroll 1
-                    for (int c = 0; c < 3; ++c) {
-                        const floatx4 n = mfma16<T>(class_part(vf, c), seen, zero);
+            for (int nt = 0; nt < NT; ++nt) {
+                float x[4];
+                hidden4<T, D, Q8>(P, row, 16 * nt + 4 * g, x);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) add[r] += n[r] > 0.f ? (c == 0 ? INFINITY : c == 1 ? -INFINITY : NAN) : 0.f;
-                    }
-                }
-                o_acc[mt][nt] = o + add;
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o_acc[mt][nt][j] += key <= lim[mt] ? x[j] : 0.f;
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -302,6 +328,237 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
     }
 }
 
+// Many rows (a prompt's chunk, a wide tree of shared heads): bound by the matrix products and the exponentials between them.  A
+// workgroup's four waves hold 32 rows each and share 64-key tiles of K and V in LDS (two buffers: the next tile's rows travel
+// global -> registers while this one is computed, registers -> LDS behind it; one barrier a tile).  With 32 x 32 products,
+//   S^T = K Q^T    leaves a lane with 32 scores of ONE row: its maximum and sum are lane-local but for one exchange between the
+//                  two half-waves, and the weights are the second product's B operand where they stand
+//   O^T += V^T P^T V^T by transposing LDS reads; a lane's outputs belong to the same row: rescaling is lane-local, and skipped
+//                  while no maximum of the wave moves.
+// Two workgroups share a CU, so that one's exponentials run beside the other's products.
+#define PAT_NW 4
+#define PAT_BK 64
+template <typename T, int D, bool Q8>
+__global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(PagedAttnParams P) {
+    typedef typename vec_of<T>::v8 v8;
+    typedef typename vec_of<T>::v4 v4;
+    constexpr int EPL = Q8 ? 16 : 8, LPR = D / EPL, RPP = PAT_NW * 64 / LPR, PASSES = PAT_BK / RPP;
+    constexpr int KSTR = D + 8, VSTR = D + 32;      // 16-byte reads of 16 rows, 8-byte transposing reads of 4 rows: all banks once
+    constexpr int BUF = PAT_BK * (KSTR + VSTR);     // elements
+    constexpr int QS = D / 16, NB = D / 32, KS = PAT_BK / 16, ROWS = 32 * PAT_NW;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF * 2];
+    __shared__ int lds_hidden[2][PAT_BK];           // rows of a tile with values that were taken out
+    AttnItem I;
+    if (!attn_item(P, ROWS, I)) return;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, qc = lane & 31, h = lane >> 5;
+    const int k0 = I.split * P.split_len, k1 = I.end < k0 + P.split_len ? I.end : k0 + P.split_len;
+
+    const int wrow = I.row0 + 32 * wave;            // the wave's first row
+    int r = wrow + qc;
+    const bool live = r < I.rows;
+    r = live ? r : I.rows - 1;
+    const int token = r / P.group, head = I.kvh * P.group + r - token * P.group;
+    int lim = I.past + token;                       // last key this lane's row sees, here
+    lim = lim < k1 ? lim : k1 - 1;
+    v8 qf[QS];
+    {
+        const T* qr = (const T*)P.q + head * P.q_head_stride + (size_t)(I.first + token) * P.q_row_stride + 8 * h;
+#pragma unroll
+        for (int s = 0; s < QS; ++s) qf[s] = *(const v8*)(qr + 16 * s);
+    }
+    const int lim_of_row0 = I.past + I.row0 / P.group;
+    int wlast = wrow + 31 < I.rows ? wrow + 31 : I.rows - 1;
+    int lim_lo = I.past + wrow / P.group, lim_hi = I.past + wlast / P.group;
+    lim_lo = wrow < I.rows ? (lim_lo < k1 ? lim_lo : k1 - 1) : -1;      // a wave without rows only helps to fetch
+    lim_hi = wrow < I.rows ? (lim_hi < k1 ? lim_hi : k1 - 1) : -1;
+
+    float m_run = -INFINITY, l_run = 0.f;
+    floatx16 o_acc[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o_acc[i] = floatx16{};
+
+    u32x4 kr[PASSES], vr[PASSES];
+    uint32_t ksr[PASSES], vsr[PASSES];
+    int pg[PASSES];
+    const int lrow = tid / LPR, lcol = tid % LPR;
+    auto pages = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int p = page_of(P.map, I.seq, (key0 + i * RPP + lrow) >> P.map.shift);
+            pg[i] = p < 0 ? 0 : p;                  // behind a table that ends early: in bounds, weight 0
+        }
+    };
+    auto load = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int key = key0 + i * RPP + lrow;
+            const size_t row = stored_row(P, pg[i], I.kvh, key);
+            const size_t at = row * D * (Q8 ? 1 : 2) + 16 * lcol;
+            kr[i] = *(const u32x4*)((const uint8_t*)P.k + at);
+            vr[i] = *(const u32x4*)((const uint8_t*)P.v + at);
+            if constexpr (Q8) { ksr[i] = P.ks[row]; vsr[i] = P.vs[row]; }
+        }
+    };
+    const int lim0 = lim_of_row0 < k1 ? lim_of_row0 : k1 - 1;           // keys up to here are seen by every row of the workgroup
+    auto stage = [&](int key0, int which) {
+        T *bk = (T*)lds + which * BUF, *bv = bk + PAT_BK * KSTR;
+        const bool masked = key0 + PAT_BK - 1 > lim0;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int rr = i * RPP + lrow;
+            if (masked && key0 + rr >= k1) { vr[i] = u32x4{0, 0, 0, 0}; vsr[i] = 127; }      // rows behind the end hold anything
+            bool bad = false;
+            if constexpr (Q8) {
+                v8 lo, hi;
+                e4m3_expand<T>(kr[i], e4m3_scale(ksr[i]), lo, hi);
+                *(v8*)(bk + rr * KSTR + 16 * lcol) = lo;
+                *(v8*)(bk + rr * KSTR + 16 * lcol + 8) = hi;
+                e4m3_expand<T>(vr[i], e4m3_scale(vsr[i]), lo, hi);
+                if (masked) bad = take_nonfinite<T>(lo) | take_nonfinite<T>(hi);
+                *(v8*)(bv + rr * VSTR + 16 * lcol) = lo;
+                *(v8*)(bv + rr * VSTR + 16 * lcol + 8) = hi;
+            } else {
+                *(u32x4*)(bk + rr * KSTR + 8 * lcol) = kr[i];
+                v8 w = __builtin_bit_cast(v8, vr[i]);
+                if (masked) bad = take_nonfinite<T>(w);
+                *(v8*)(bv + rr * VSTR + 8 * lcol) = w;
+            }
+            if (masked) {
+                const uint64_t lanes = __ballot(bad);
+                if (lcol == 0) lds_hidden[which][rr] = (lanes >> (lane & ~(LPR - 1))) & ((1ull << LPR) - 1) ? 1 : 0;
+            }
+        }
+    };
+    auto compute = [&](int key0, int which, auto masked_t) {
+        constexpr bool MASKED = decltype(masked_t)::value;
+        const T *bk = (const T*)lds + which * BUF, *bv = bk + PAT_BK * KSTR;
+        floatx16 s_acc[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            floatx16 acc = {};
+#pragma unroll
+            for (int s = 0; s < QS; ++s) acc = mfma32<T>(*(const v8*)(bk + (32 * b + qc) * KSTR + 16 * s + 8 * h), qf[s], acc);
+            s_acc[b] = acc;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if constexpr (MASKED) {
+                    const int key = key0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
+                    s_acc[b][i] = key <= lim ? s_acc[b][i] : -INFINITY;
+                }
+                mx = fmaxf(mx, s_acc[b][i]);
+            }
+        {
+            unsigned a = __builtin_bit_cast(unsigned, mx), c = a;
+            lane_swap32(a, c);
+            mx = fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, c));
+        }
+        const float m_new = fmaxf(m_run, mx * P.scale_log2e);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        if (__any(m_new > m_run)) {
+            const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+            l_run *= alpha;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o_acc[b][i] *= alpha;
+            m_run = m_new;
+        }
+        v8 pf[KS];
+        float sum = 0.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s_acc[b][i], P.scale_log2e, -m_use));
+                sum += p;
+                pf[2 * b + (i >> 3)][i & 7] = (T)p;
+            }
+        l_run += sum;
+        // slot (h, j) of step ks is key 16 ks + 8 (j >> 2) + 4 h + (j & 3): the order the weights stand in
+        auto v_frag = [&](int ks, int b) {
+            const T* a = bv + (16 * ks + 4 * h + ((lane & 15) >> 2)) * VSTR + 32 * b + (lane & 16) + 4 * (lane & 3);
+            const u32x2 lo = read_transposed(a), hi = read_transposed(a + 8 * VSTR);
+            return __builtin_bit_cast(v8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+        };
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o_acc[b] = mfma32<T>(v_frag(ks, b), pf[ks], o_acc[b]);
+        if (key0 + PAT_BK - 1 <= lim0) return;
+        uint64_t hidden = __ballot(lds_hidden[which][lane] != 0);
+        while (hidden) {                            // wave-uniform, and hardly ever entered
+            const int key = key0 + __builtin_ctzll(hidden), page = page_of(P.map, I.seq, key >> P.map.shift);
+            hidden &= hidden - 1;
+            const size_t row = stored_row(P, page < 0 ? 0 : page, I.kvh, key);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x[4];
+                    hidden4<T, D, Q8>(P, row, 32 * b + 8 * i + 4 * h, x);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o_acc[b][4 * i + j] += key <= lim ? x[j] : 0.f;
+                }
+        }
+    };
+
+    if (k0 < k1) {
+        pages(k0);
+        load(k0);
+        if (k0 + PAT_BK < k1) pages(k0 + PAT_BK);
+        stage(k0, 0);
+    }
+    int cur = 0;
+    for (int key0 = k0; key0 < k1; key0 += PAT_BK, cur ^= 1) {
+        __syncthreads();
+        const int nxt = key0 + PAT_BK;
+        if (nxt < k1) {
+            load(nxt);
+            if (nxt + PAT_BK < k1) pages(nxt + PAT_BK);
+        }
+        if (key0 + PAT_BK - 1 <= lim_lo) compute(key0, cur, std::false_type{});
+        else if (key0 <= lim_hi) compute(key0, cur, std::true_type{});
+        if (nxt < k1) stage(nxt, cur ^ 1);
+    }
+
+    {
+        unsigned a = __builtin_bit_cast(unsigned, l_run), c = a;
+        lane_swap32(a, c);
+        l_run = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, c);
+    }
+    if (!live) return;
+    if (I.n_parts <= 1) {
+        const float inv = l_run != 0.f ? 1.0f / l_run : 0.f;        // a row that sees nothing: zeros
+        T* dst = (T*)P.out + (size_t)(I.first + token) * P.out_stride + (size_t)head * D + 4 * h;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v4 w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (T)(o_acc[b][4 * i + j] * inv);
+                *(v4*)(dst + 32 * b + 8 * i) = w;
+            }
+    } else {
+        const size_t pr = ((size_t)I.split * P.n_rows + I.first + token) * P.n_heads + head;
+        float* dst = P.part_o + pr * D + 4 * h;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                floatx4 w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = o_acc[b][4 * i + j];
+                *(floatx4*)(dst + 32 * b + 8 * i) = w;
+            }
+        if (h == 0) { P.part_ml[pr * 2] = m_run; P.part_ml[pr * 2 + 1] = l_run; }
+    }
+}
+
 // Joins the parts of the key axis: one workgroup a (row, head), its waves take the parts in turn.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_attention_join_kernel(PagedAttnParams P, int tile_rows) {
@@ -343,7 +600,7 @@ struct AttnPlan { int tile_rows, n_tiles, n_splits, split_len; };
 static AttnPlan attn_plan(int n_seqs, int max_rows, int max_len, int n_heads, int h_kv) {
     AttnPlan A;
     const int rows = max_rows * (n_heads / h_kv);
-    A.tile_rows = rows <= 16 ? 16 : 32;
+    A.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
     A.n_tiles = (rows + A.tile_rows - 1) / A.tile_rows;
     const int64_t base = (int64_t)n_seqs * h_kv * A.n_tiles;
     int64_t want = (2048 + base - 1) / base;
@@ -390,12 +647,14 @@ extern "C" int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t 
                          need ? (float*)workspace + (size_t)A.n_splits * n_rows * n_heads * d : nullptr};
     hipStream_t st = (hipStream_t)stream;
 #define SQ_A(TT, DD, QQ, MM) hipLaunchKernelGGL((paged_attention_rows_kernel<TT, DD, QQ, MM>), dim3((unsigned)grid), dim3(PAD_NW * 64), 0, st, P)
-#define SQ_AM(TT, DD, QQ) do { if (A.tile_rows == 16) SQ_A(TT, DD, QQ, 1); else SQ_A(TT, DD, QQ, 2); } while (0)
+#define SQ_AT(TT, DD, QQ) hipLaunchKernelGGL((paged_attention_tiles_kernel<TT, DD, QQ>), dim3((unsigned)grid), dim3(PAT_NW * 64), 0, st, P)
+#define SQ_AM(TT, DD, QQ) do { if (A.tile_rows == 16) SQ_A(TT, DD, QQ, 1); else if (A.tile_rows == 32) SQ_A(TT, DD, QQ, 2); else SQ_AT(TT, DD, QQ); } while (0)
 #define SQ_AD(TT, DD) do { if (k_scales) SQ_AM(TT, DD, true); else SQ_AM(TT, DD, false); } while (0)
     if (dtype == SQ_DTYPE_F16) { if (d == 128) SQ_AD(half_t, 128); else SQ_AD(half_t, 64); }
     else                       { if (d == 128) SQ_AD(bf16_t, 128); else SQ_AD(bf16_t, 64); }
 #undef SQ_AD
 #undef SQ_AM
+#undef SQ_AT
 #undef SQ_A
     int rc = sq_check_launch();
     if (rc != SQ_OK || A.n_splits <= 1) return rc;
