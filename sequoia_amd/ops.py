@@ -35,13 +35,13 @@ def _need(t: torch.Tensor, dtype, name: str, contiguous: bool = True):
 _DTYPE_CODES = {torch.float16: native.SQ_DTYPE_F16, torch.bfloat16: native.SQ_DTYPE_BF16, torch.float32: native.SQ_DTYPE_F32}
 
 
-def _on_device(dev, **tensors):
-    """Every tensor on the device `dev` of the call (None is allowed): the launch goes to that device's current stream."""
+def _on_device(dev, *tensors):
+    """Every tensor (None is allowed) on the device `dev` of the call: the launch goes to that device's current stream."""
     if dev.type != "cuda":
         raise native.SequoiaNativeError(f"the tensors live on {dev}: the paged path only runs on a HIP device (no CPU fallback)")
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name}: lives on {t.device}, the call's tensors on {dev}")
+    for t in tensors:
+        if t is not None and t.get_device() != dev.index:
+            raise ValueError(f"the call's tensors live on different devices: {[str(x.device) for x in tensors if x is not None]} beside {dev}")
 
 
 def _index(t, dtype, n, name):
@@ -421,13 +421,15 @@ class HipOps:
         return result
 
     # ---- batched speculative decoding over a paged KV cache -------------------------------------
-    def _launch(self, dev, fn, what, args):
+    @staticmethod
+    def _launch(dev, fn, what, args):
         """fn(*args, stream) on `dev`'s current stream, with `dev` current for the launch."""
+        # the raw handle: torch.cuda.current_stream() builds a Stream object, 2.7 us of a small call's 13
         if dev.index == torch.cuda.current_device():
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
         else:
             with torch.cuda.device(dev):
-                rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
         if rc:
             check(rc, what)
 
@@ -438,8 +440,7 @@ class HipOps:
         [n_pages, H_kv, page_size, D] in qkv's type, or float8_e4m3fn with k_scales / v_scales (uint8, [n_pages, H_kv, page_size]).
         Rows behind cu_rows[-1] are left alone."""
         dev, dt = qkv.device, qkv.dtype
-        _on_device(dev, q_out=q_out, k_pages=k_pages, v_pages=v_pages, cos=cos, sin=sin, position_ids=position_ids, page_table=page_table,
-                   seq_lens=seq_lens, cu_rows=cu_rows, k_scales=k_scales, v_scales=v_scales)
+        _on_device(dev, q_out, k_pages, v_pages, cos, sin, position_ids, page_table, seq_lens, cu_rows, k_scales, v_scales)
         if dt not in (torch.float16, torch.bfloat16):
             raise TypeError(f"qkv: expected torch.float16 or torch.bfloat16, got {dt}")
         for t, name in ((q_out, "q_out"), (cos, "cos"), (sin, "sin")):
@@ -468,8 +469,7 @@ class HipOps:
         [sequences, H_kv, M, D] (fp16 or bf16, rows contiguous: layer slabs of static caches fit).  Other rows stay as they are.
         max_count: no sequence asks for more rows (default: M); rows beyond it are not read."""
         dev, dt = k_out.device, k_out.dtype
-        _on_device(dev, k_pages=k_pages, v_pages=v_pages, v_out=v_out, page_table=page_table, starts=starts, counts=counts,
-                   k_scales=k_scales, v_scales=v_scales)
+        _on_device(dev, k_pages, v_pages, v_out, page_table, starts, counts, k_scales, v_scales)
         if dt not in (torch.float16, torch.bfloat16) or v_out.dtype != dt:
             raise TypeError(f"k_out / v_out: expected torch.float16 or torch.bfloat16 twice, got {dt}, {v_out.dtype}")
         n_pages, h_kv, page_size, d, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
@@ -498,8 +498,7 @@ class HipOps:
         behind more keys (defaults: n_rows, the table's whole width); they size the launch, and rows and keys beyond them are left
         out.  The default max_len costs workgroups that find nothing to do."""
         dev, dt = q.device, q.dtype
-        _on_device(dev, k_pages=k_pages, v_pages=v_pages, out=out, page_table=page_table, seq_lens=seq_lens, cu_rows=cu_rows,
-                   k_scales=k_scales, v_scales=v_scales)
+        _on_device(dev, k_pages, v_pages, out, page_table, seq_lens, cu_rows, k_scales, v_scales)
         if dt not in (torch.float16, torch.bfloat16) or out.dtype != dt:
             raise TypeError(f"q / out: expected torch.float16 or torch.bfloat16 twice, got {dt}, {out.dtype}")
         n_pages, h_kv, page_size, d, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
@@ -535,8 +534,7 @@ class HipOps:
         (-1: the deciding row is no distribution)."""
         dev, dt = target_logits.device, target_logits.dtype
         temps = temperature if isinstance(temperature, torch.Tensor) else None
-        _on_device(dev, draft_logits=draft_logits, draft_tokens=draft_tokens, cu_drafts=cu_drafts, u_accept=u_accept, u_next=u_next,
-                   temperature=temps, n_accepted=n_accepted, next_tokens=next_tokens)
+        _on_device(dev, draft_logits, draft_tokens, cu_drafts, u_accept, u_next, temps, n_accepted, next_tokens)
         if dt not in _DTYPE_CODES or draft_logits.dtype != dt:
             raise TypeError(f"target_logits / draft_logits: expected fp16, bf16 or fp32 twice, got {dt}, {draft_logits.dtype}")
         n_seqs, n_drafts = n_accepted.shape[0], draft_tokens.shape[0]
