@@ -38,6 +38,18 @@ static inline int page_shift(int page_size) {
     return -1;
 }
 
+// A table entry by wave-uniform index, loaded without a branch and looked at only where it is used (check_page), so that the wait
+// for it falls behind the loads issued after it; one that is no page of the pool (only behind a table that ends early) becomes
+// page 0, in bounds.
+__device__ __forceinline__ int page_entry(const PageMap& M, int seq, int i) {
+    i = i < M.width - 1 ? i : M.width - 1;
+    return M.table[(size_t)seq * M.width + (i > 0 ? i : 0)];
+}
+__device__ __forceinline__ int check_page(const PageMap& M, int entry) {
+    const int p = __builtin_amdgcn_readfirstlane(entry);
+    return (unsigned)p < (unsigned)M.n_pages ? p : 0;
+}
+
 // the sequence that row `t` of a ragged batch belongs to (n_seqs: none), by one wave: cu_rows is ascending, so it is the number
 // of sequences that end at or before t.  64 ends a load instead of a search's chain of dependent ones.
 __device__ __forceinline__ int seq_of_row(const int32_t* cu_rows, int n_seqs, int t) {

@@ -6,7 +6,6 @@
 // head r % group), so that every stored row is read once for all of them.
 #include "paged.h"
 #include "attn_map.h"
-#include <type_traits>
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef __fp16 fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
@@ -86,13 +85,13 @@ __device__ __forceinline__ bool attn_item(const PagedAttnParams& P, int tile_row
     I.seq = u / P.h_kv; I.kvh = u - I.seq * P.h_kv;
     const int tile = P.n_tiles - 1 - w / P.n_splits;
     I.split = w % P.n_splits;
-    I.first = P.cu_rows[I.seq];
-    int n = P.cu_rows[I.seq + 1] - I.first;
+    I.first = __builtin_amdgcn_readfirstlane(P.cu_rows[I.seq]);        // scalar registers: what branches on these is uniform
+    const int n = __builtin_amdgcn_readfirstlane(P.cu_rows[I.seq + 1]) - I.first;
+    I.past = __builtin_amdgcn_readfirstlane(P.seq_lens[I.seq]);
     if (I.first < 0 || I.first + n > P.n_rows) return false;
     I.rows = n * P.group;
     I.row0 = tile * tile_rows;
     if (I.row0 >= I.rows) return false;
-    I.past = P.seq_lens[I.seq];
     I.end = attn_tile_end(P, I.past, I.rows, tile, tile_rows);
     I.n_parts = (I.end + P.split_len - 1) / P.split_len;
     return I.split < I.n_parts || (I.split == 0 && I.n_parts == 0);
@@ -122,7 +121,7 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
     __shared__ float lds_ml[PAD_NW][ROWS][2];
     AttnItem I;
     if (!attn_item(P, ROWS, I)) return;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, qc = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, qc = lane & 15, g = lane >> 4;
     const int k0 = I.split * P.split_len, k1 = I.end < k0 + P.split_len ? I.end : k0 + P.split_len;
     T* my_k = (T*)(lds + wave * WAVE_BYTES);
     T* my_v = my_k + PAD_BK * KSTR;
@@ -153,30 +152,31 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
     u32x4 kr[PASSES], vr[PASSES];
     uint32_t ksr[PASSES], vsr[PASSES];
     const int lrow = lane / LPR, lcol = lane % LPR;
-    // pages of the two 16-row halves of a chunk; a missing one (only behind a table that ends early) reads page 0, in bounds
+    // entries of the pages that hold the two 16-row halves of a chunk
     auto pages = [&](int key0, int& a, int& b) {
-        a = page_of(P.map, I.seq, key0 >> P.map.shift);
-        b = page_of(P.map, I.seq, (key0 + 16) >> P.map.shift);
-        a = a < 0 ? 0 : a; b = b < 0 ? 0 : b;
+        a = page_entry(P.map, I.seq, key0 >> P.map.shift);
+        b = page_entry(P.map, I.seq, (key0 + 16) >> P.map.shift);
     };
-    auto load = [&](int key0, int pa, int pb) {
+    auto load = [&](int key0, int ea, int eb) {
+        const size_t ra = stored_row(P, check_page(P.map, ea), I.kvh, key0), rb = stored_row(P, check_page(P.map, eb), I.kvh, key0 + 16);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            const int rr = i * RPP + lrow;
-            const size_t r = stored_row(P, i * RPP < 16 ? pa : pb, I.kvh, key0 + rr);
-            const size_t at = r * D * (Q8 ? 1 : 2) + 16 * lcol;
-            kr[i] = *(const u32x4*)((const uint8_t*)P.k + at);
-            vr[i] = *(const u32x4*)((const uint8_t*)P.v + at);
-            if constexpr (Q8) { ksr[i] = P.ks[r]; vsr[i] = P.vs[r]; }
+            const size_t r = i * RPP < 16 ? ra + i * RPP : rb + (i * RPP - 16);         // scalar
+            const uint32_t at = lane * 16;                                              // rows lie one behind the other
+            kr[i] = *(const u32x4*)((const uint8_t*)P.k + r * (D * (Q8 ? 1 : 2)) + at);
+            vr[i] = *(const u32x4*)((const uint8_t*)P.v + r * (D * (Q8 ? 1 : 2)) + at);
+            if constexpr (Q8) { ksr[i] = (P.ks + r)[lrow]; vsr[i] = (P.vs + r)[lrow]; }
         }
     };
-    int key0 = k0 + wave * PAD_BK, pa = 0, pb = 0;
+    constexpr int STEP = PAD_NW * PAD_BK;
+    int key0 = k0 + wave * PAD_BK, ea = 0, eb = 0;
     if (key0 < k1) {
-        pages(key0, pa, pb);
-        load(key0, pa, pb);
-        if (key0 + PAD_NW * PAD_BK < k1) pages(key0 + PAD_NW * PAD_BK, pa, pb);
+        int fa, fb;
+        pages(key0, fa, fb);
+        pages(key0 + STEP, ea, eb);
+        load(key0, fa, fb);
     }
-    for (; key0 < k1; key0 += PAD_NW * PAD_BK) {
+    for (; key0 < k1; key0 += STEP) {
         const bool tail = key0 + PAD_BK > k1;       // rows behind the end hold anything: their weights are 0, and so are they
         const bool masked = tail || key0 + PAD_BK - 1 > lim0;
         uint32_t hidden = 0;                        // rows of the chunk with values that were taken out
@@ -207,10 +207,10 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
                     for (int j = 0; j < RPP; ++j) hidden |= (uint32_t)(((lanes >> (j * LPR)) & ((1ull << LPR) - 1)) != 0) << (i * RPP + j);
             }
         }
-        const int nxt = key0 + PAD_NW * PAD_BK;
-        if (nxt < k1) {
-            load(nxt, pa, pb);
-            if (nxt + PAD_NW * PAD_BK < k1) pages(nxt + PAD_NW * PAD_BK, pa, pb);
+        if (key0 + STEP < k1) {                     // the entries of the chunk after the next come first: loads end in order
+            const int fa = ea, fb = eb;
+            pages(key0 + 2 * STEP, ea, eb);
+            load(key0 + STEP, fa, fb);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -229,24 +229,29 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
             }
         }
         v8 pf[MT];
-        float alpha[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             float sv[8], cmax = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float x = s_acc[mt][j >> 2][j & 3] * P.scale_log2e;
-                if (masked) {
-                    const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                    x = key < k1 && key <= lim[mt] ? x : -INFINITY;
-                }
-                sv[j] = x;
-                cmax = fmaxf(cmax, x);
+            for (int j = 0; j < 8; ++j) sv[j] = s_acc[mt][j >> 2][j & 3] * P.scale_log2e;
+            if (masked) {
+                int seen = (lim[mt] < k1 ? lim[mt] : k1 - 1) - key0 - 4 * g;       // opaque: not eight differences kept over the loop
+                asm("" : "+v"(seen));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sv[j] = 16 * (j >> 2) + (j & 3) <= seen ? sv[j] : -INFINITY;
             }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) cmax = fmaxf(cmax, sv[j]);
             cmax = group4_max(cmax);
             const float m_new = fmaxf(m_run[mt], cmax);
             const float m_use = m_new == -INFINITY ? 0.f : m_new;       // nothing seen so far
-            alpha[mt] = __builtin_amdgcn_exp2f(m_run[mt] - m_use);
+            if (__any(m_new > m_run[mt])) {
+                const float alpha = __builtin_amdgcn_exp2f(m_run[mt] - m_use);
+                l_run[mt] *= alpha;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) o_acc[mt][nt] *= alpha;
+                m_run[mt] = m_new;
+            }
             float psum = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -254,8 +259,7 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
                 psum += p;
                 pf[mt][j] = (T)p;
             }
-            l_run[mt] = l_run[mt] * alpha[mt] + psum;
-            m_run[mt] = m_new;
+            l_run[mt] += psum;
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -265,17 +269,12 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
             const u32x2 lo = read_transposed(a0), hi = read_transposed(a0 + 16 * VSTR);
             const v8 vf = __builtin_bit_cast(v8, u32x4{lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                floatx4 o = o_acc[mt][nt];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] *= alpha[mt];
-                o_acc[mt][nt] = mfma16<T>(vf, pf[mt], o);
-            }
+            for (int mt = 0; mt < MT; ++mt) o_acc[mt][nt] = mfma16<T>(vf, pf[mt], o_acc[mt][nt]);
         }
         while (hidden) {                            // wave-uniform, and hardly ever entered
-            const int key = key0 + __builtin_ctz(hidden), page = page_of(P.map, I.seq, key >> P.map.shift);
+            const int key = key0 + __builtin_ctz(hidden);
             hidden &= hidden - 1;
-            const size_t row = stored_row(P, page < 0 ? 0 : page, I.kvh, key);
+            const size_t row = stored_row(P, check_page(P.map, page_entry(P.map, I.seq, key >> P.map.shift)), I.kvh, key);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float x[4];
@@ -350,7 +349,7 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     __shared__ int lds_hidden[2][PAT_BK];           // rows of a tile with values that were taken out
     AttnItem I;
     if (!attn_item(P, ROWS, I)) return;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, qc = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, qc = lane & 31, h = lane >> 5;
     const int k0 = I.split * P.split_len, k1 = I.end < k0 + P.split_len ? I.end : k0 + P.split_len;
 
     const int wrow = I.row0 + 32 * wave;            // the wave's first row
@@ -381,22 +380,22 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     uint32_t ksr[PASSES], vsr[PASSES];
     int pg[PASSES];
     const int lrow = tid / LPR, lcol = tid % LPR;
+    // a wave's rows of a pass lie in one 16-row block, so in one page: its entry is uniform, the rows one behind the other
+    constexpr int RPW = 64 / LPR;
     auto pages = [&](int key0) {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int p = page_of(P.map, I.seq, (key0 + i * RPP + lrow) >> P.map.shift);
-            pg[i] = p < 0 ? 0 : p;                  // behind a table that ends early: in bounds, weight 0
-        }
+        for (int i = 0; i < PASSES; ++i) pg[i] = page_entry(P.map, I.seq, (key0 + i * RPP + wave * RPW) >> P.map.shift);
     };
-    auto load = [&](int key0) {
+    auto load = [&](int key0) {                     // takes the entries, and asks for those of the next tile first: loads end in order
+        size_t row[PASSES];
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) row[i] = stored_row(P, check_page(P.map, pg[i]), I.kvh, key0 + i * RPP + wave * RPW);
+        pages(key0 + PAT_BK);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            const int key = key0 + i * RPP + lrow;
-            const size_t row = stored_row(P, pg[i], I.kvh, key);
-            const size_t at = row * D * (Q8 ? 1 : 2) + 16 * lcol;
-            kr[i] = *(const u32x4*)((const uint8_t*)P.k + at);
-            vr[i] = *(const u32x4*)((const uint8_t*)P.v + at);
-            if constexpr (Q8) { ksr[i] = P.ks[row]; vsr[i] = P.vs[row]; }
+            kr[i] = *(const u32x4*)((const uint8_t*)P.k + row[i] * (D * (Q8 ? 1 : 2)) + lane * 16);
+            vr[i] = *(const u32x4*)((const uint8_t*)P.v + row[i] * (D * (Q8 ? 1 : 2)) + lane * 16);
+            if constexpr (Q8) { ksr[i] = (P.ks + row[i])[lane / LPR]; vsr[i] = (P.vs + row[i])[lane / LPR]; }
         }
     };
     const int lim0 = lim_of_row0 < k1 ? lim_of_row0 : k1 - 1;           // keys up to here are seen by every row of the workgroup
@@ -429,8 +428,7 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
             }
         }
     };
-    auto compute = [&](int key0, int which, auto masked_t) {
-        constexpr bool MASKED = decltype(masked_t)::value;
+    auto compute = [&](int key0, int which, bool masked) {
         const T *bk = (const T*)lds + which * BUF, *bv = bk + PAT_BK * KSTR;
         floatx16 s_acc[2];
 #pragma unroll
@@ -440,17 +438,19 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
             for (int s = 0; s < QS; ++s) acc = mfma32<T>(*(const v8*)(bk + (32 * b + qc) * KSTR + 16 * s + 8 * h), qf[s], acc);
             s_acc[b] = acc;
         }
+        if (masked) {
+            int seen = lim - key0 - 4 * h;          // opaque, or the 32 differences to it are kept in registers over the whole loop
+            asm("" : "+v"(seen));
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s_acc[b][i] = 32 * b + 8 * (i >> 2) + (i & 3) <= seen ? s_acc[b][i] : -INFINITY;
+        }
         float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if constexpr (MASKED) {
-                    const int key = key0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
-                    s_acc[b][i] = key <= lim ? s_acc[b][i] : -INFINITY;
-                }
-                mx = fmaxf(mx, s_acc[b][i]);
-            }
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s_acc[b][i]);
         {
             unsigned a = __builtin_bit_cast(unsigned, mx), c = a;
             lane_swap32(a, c);
@@ -491,9 +491,9 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
         if (key0 + PAT_BK - 1 <= lim0) return;
         uint64_t hidden = __ballot(lds_hidden[which][lane] != 0);
         while (hidden) {                            // wave-uniform, and hardly ever entered
-            const int key = key0 + __builtin_ctzll(hidden), page = page_of(P.map, I.seq, key >> P.map.shift);
+            const int key = key0 + __builtin_ctzll(hidden);
             hidden &= hidden - 1;
-            const size_t row = stored_row(P, page < 0 ? 0 : page, I.kvh, key);
+            const size_t row = stored_row(P, check_page(P.map, page_entry(P.map, I.seq, key >> P.map.shift)), I.kvh, key);
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -509,19 +509,14 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     if (k0 < k1) {
         pages(k0);
         load(k0);
-        if (k0 + PAT_BK < k1) pages(k0 + PAT_BK);
         stage(k0, 0);
     }
     int cur = 0;
     for (int key0 = k0; key0 < k1; key0 += PAT_BK, cur ^= 1) {
         __syncthreads();
         const int nxt = key0 + PAT_BK;
-        if (nxt < k1) {
-            load(nxt);
-            if (nxt + PAT_BK < k1) pages(nxt + PAT_BK);
-        }
-        if (key0 + PAT_BK - 1 <= lim_lo) compute(key0, cur, std::false_type{});
-        else if (key0 <= lim_hi) compute(key0, cur, std::true_type{});
+        if (nxt < k1) load(nxt);
+        if (key0 <= lim_hi) compute(key0, cur, key0 + PAT_BK - 1 > lim_lo);
         if (nxt < k1) stage(nxt, cur ^ 1);
     }
 
