@@ -10,6 +10,10 @@
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef __fp16 fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
 
+// Values loaded before a loop are waited for before it: left to the loop, the wait for them is repeated in every trip, and there it
+// is a wait for the trip's own prefetch.
+template <typename V> __device__ __forceinline__ void arrived(V& v) { asm volatile("" : "+v"(v)); }
+
 struct PagedAttnParams {
     const void* q; int64_t q_head_stride, q_row_stride;
     const void *k, *v;
@@ -68,6 +72,13 @@ template <typename T, int D, bool Q8> __device__ __forceinline__ void hidden4(co
         for (int j = 0; j < 4; ++j) x[j] = __builtin_fabsf((float)w[j]) < INFINITY ? 0.f : (float)w[j];
     }
 }
+
+// 16 bytes a lane from base + from (base uniform) to LDS byte to + 16 * lane (uniform).  By hand, because the compiler takes any LDS
+// read for one of what such a load writes, and waits for all of them in front of it: who reads the bytes calls loads_done() first.
+__device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(from), "s"(base), "s"(to) : "memory");      // (m0 is nobody else's here)
+}
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // what a workgroup works on
 struct AttnItem {
@@ -176,6 +187,10 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
         pages(key0 + STEP, ea, eb);
         load(key0, fa, fb);
     }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int s = 0; s < DSTEPS; ++s) arrived(qf[mt][s]);
     for (; key0 < k1; key0 += STEP) {
         const bool tail = key0 + PAD_BK > k1;       // rows behind the end hold anything: their weights are 0, and so are they
         const bool masked = tail || key0 + PAD_BK - 1 > lim0;
@@ -342,10 +357,9 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     typedef typename vec_of<T>::v8 v8;
     typedef typename vec_of<T>::v4 v4;
     constexpr int EPL = Q8 ? 16 : 8, LPR = D / EPL, RPP = PAT_NW * 64 / LPR, PASSES = PAT_BK / RPP;
-    constexpr int KSTR = D + 8, VSTR = D + 32;      // 16-byte reads of 16 rows, 8-byte transposing reads of 4 rows: all banks once
-    constexpr int BUF = PAT_BK * (KSTR + VSTR);     // elements
+    constexpr int BUF = 2 * PAT_BK * D;             // elements: K, then V
     constexpr int QS = D / 16, NB = D / 32, KS = PAT_BK / 16, ROWS = 32 * PAT_NW;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF * 2];
+    __shared__ __attribute__((aligned(256))) unsigned char lds[2 * BUF * 2];
     __shared__ int lds_hidden[2][PAT_BK];           // rows of a tile with values that were taken out
     AttnItem I;
     if (!attn_item(P, ROWS, I)) return;
@@ -376,66 +390,97 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
 #pragma unroll
     for (int i = 0; i < NB; ++i) o_acc[i] = floatx16{};
 
-    u32x4 kr[PASSES], vr[PASSES];
-    uint32_t ksr[PASSES], vsr[PASSES];
-    int pg[PASSES];
-    const int lrow = tid / LPR, lcol = tid % LPR;
+    // Rows lie in LDS one behind the other, their 16-byte chunks in an order that depends on the row: chunk c of row r is at
+    // place c ^ order(r).  The reads of K (one chunk of 16 consecutive rows) and the transposing reads of V (four chunks of four
+    // consecutive rows) then touch every bank once, and rows can be fetched by loads that write LDS themselves.
+    auto k_order = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+    auto v_order = [](int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 2) << 1) | ((r >> 2) & 3); };
+    const int lim0 = lim_of_row0 < k1 ? lim_of_row0 : k1 - 1;           // keys up to here are seen by every row of the workgroup
+    const int lrow = lane / LPR, lcol = lane % LPR;
     // a wave's rows of a pass lie in one 16-row block, so in one page: its entry is uniform, the rows one behind the other
     constexpr int RPW = 64 / LPR;
+    int pg[PASSES];
     auto pages = [&](int key0) {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) pg[i] = page_entry(P.map, I.seq, (key0 + i * RPP + wave * RPW) >> P.map.shift);
     };
-    auto load = [&](int key0) {                     // takes the entries, and asks for those of the next tile first: loads end in order
-        size_t row[PASSES];
+    auto rows_of = [&](int key0, size_t (&row)[PASSES]) {   // takes the entries, and asks for those of the next tile first: loads end in order
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) row[i] = stored_row(P, check_page(P.map, pg[i]), I.kvh, key0 + i * RPP + wave * RPW);
         pages(key0 + PAT_BK);
+    };
+    // values of V that are not finite, in a tile that some row does not see all of: staged as 0, and their rows noted
+    auto note = [&](int which, int rr, bool bad) {
+        const uint64_t lanes = __ballot(bad);
+        if (lcol == 0) lds_hidden[which][rr] = (lanes >> (lane & ~(LPR - 1))) & ((1ull << LPR) - 1) ? 1 : 0;
+    };
+    // e4m3: through registers, which widen
+    u32x4 kr[PASSES], vr[PASSES];
+    uint32_t ksr[PASSES], vsr[PASSES];
+    auto load_codes = [&](int key0) {
+        size_t row[PASSES];
+        rows_of(key0, row);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            kr[i] = *(const u32x4*)((const uint8_t*)P.k + row[i] * (D * (Q8 ? 1 : 2)) + lane * 16);
-            vr[i] = *(const u32x4*)((const uint8_t*)P.v + row[i] * (D * (Q8 ? 1 : 2)) + lane * 16);
-            if constexpr (Q8) { ksr[i] = (P.ks + row[i])[lane / LPR]; vsr[i] = (P.vs + row[i])[lane / LPR]; }
+            kr[i] = *(const u32x4*)((const uint8_t*)P.k + row[i] * D + lane * 16);
+            vr[i] = *(const u32x4*)((const uint8_t*)P.v + row[i] * D + lane * 16);
+            ksr[i] = (P.ks + row[i])[lrow];
+            vsr[i] = (P.vs + row[i])[lrow];
         }
     };
-    const int lim0 = lim_of_row0 < k1 ? lim_of_row0 : k1 - 1;           // keys up to here are seen by every row of the workgroup
-    auto stage = [&](int key0, int which) {
-        T *bk = (T*)lds + which * BUF, *bv = bk + PAT_BK * KSTR;
+    auto stage_codes = [&](int key0, int which) {
+        T *bk = (T*)lds + which * BUF, *bv = bk + PAT_BK * D;
         const bool masked = key0 + PAT_BK - 1 > lim0;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            const int rr = i * RPP + lrow;
+            const int rr = i * RPP + wave * RPW + lrow;
             if (masked && key0 + rr >= k1) { vr[i] = u32x4{0, 0, 0, 0}; vsr[i] = 127; }      // rows behind the end hold anything
-            bool bad = false;
-            if constexpr (Q8) {
-                v8 lo, hi;
-                e4m3_expand<T>(kr[i], e4m3_scale(ksr[i]), lo, hi);
-                *(v8*)(bk + rr * KSTR + 16 * lcol) = lo;
-                *(v8*)(bk + rr * KSTR + 16 * lcol + 8) = hi;
-                e4m3_expand<T>(vr[i], e4m3_scale(vsr[i]), lo, hi);
-                if (masked) bad = take_nonfinite<T>(lo) | take_nonfinite<T>(hi);
-                *(v8*)(bv + rr * VSTR + 16 * lcol) = lo;
-                *(v8*)(bv + rr * VSTR + 16 * lcol + 8) = hi;
-            } else {
-                *(u32x4*)(bk + rr * KSTR + 8 * lcol) = kr[i];
-                v8 w = __builtin_bit_cast(v8, vr[i]);
-                if (masked) bad = take_nonfinite<T>(w);
-                *(v8*)(bv + rr * VSTR + 8 * lcol) = w;
-            }
-            if (masked) {
-                const uint64_t lanes = __ballot(bad);
-                if (lcol == 0) lds_hidden[which][rr] = (lanes >> (lane & ~(LPR - 1))) & ((1ull << LPR) - 1) ? 1 : 0;
-            }
+            v8 lo, hi;
+            e4m3_expand<T>(kr[i], e4m3_scale(ksr[i]), lo, hi);
+            *(v8*)(bk + rr * D + 8 * ((2 * lcol) ^ k_order(rr))) = lo;
+            *(v8*)(bk + rr * D + 8 * ((2 * lcol + 1) ^ k_order(rr))) = hi;
+            e4m3_expand<T>(vr[i], e4m3_scale(vsr[i]), lo, hi);
+            if (masked) note(which, rr, take_nonfinite<T>(lo) | take_nonfinite<T>(hi));
+            *(v8*)(bv + rr * D + 8 * ((2 * lcol) ^ v_order(rr))) = lo;
+            *(v8*)(bv + rr * D + 8 * ((2 * lcol + 1) ^ v_order(rr))) = hi;
         }
     };
+    // 16-bit rows: straight into LDS, a lane's place fixed, so the lane fetches the chunk that belongs there
+    auto fetch = [&](int key0, int which) {
+        size_t row[PASSES];
+        rows_of(key0, row);
+        const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds + which * (BUF * 2);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int r0 = i * RPP + wave * RPW, rr = r0 + lrow;
+            const uint32_t from = lrow * (2 * D);
+            load_to_lds((const uint8_t*)P.k + row[i] * (2 * D), from + 16 * (lcol ^ k_order(rr)), base + r0 * (2 * D));
+            load_to_lds((const uint8_t*)P.v + row[i] * (2 * D), from + 16 * (lcol ^ v_order(rr)), base + (PAT_BK + r0) * (2 * D));
+        }
+    };
+    auto clean = [&](int key0, int which) {         // a fetched tile that some row does not see all of
+        T* bv = (T*)lds + which * BUF + PAT_BK * D;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int rr = i * RPP + wave * RPW + lrow;
+            v8* at = (v8*)(bv + rr * D + 8 * lcol);
+            v8 w = *at;
+            const bool behind = key0 + rr >= k1;    // rows behind the end hold anything
+            if (behind) w = v8{};
+            const bool bad = take_nonfinite<T>(w);
+            if (behind | bad) *at = w;
+            note(which, rr, bad);
+        }
+        __syncthreads();
+    };
     auto compute = [&](int key0, int which, bool masked) {
-        const T *bk = (const T*)lds + which * BUF, *bv = bk + PAT_BK * KSTR;
+        const T *bk = (const T*)lds + which * BUF, *bv = bk + PAT_BK * D;
         floatx16 s_acc[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             floatx16 acc = {};
 #pragma unroll
-            for (int s = 0; s < QS; ++s) acc = mfma32<T>(*(const v8*)(bk + (32 * b + qc) * KSTR + 16 * s + 8 * h), qf[s], acc);
+            for (int s = 0; s < QS; ++s) acc = mfma32<T>(*(const v8*)(bk + (32 * b + qc) * D + 8 * ((2 * s + h) ^ k_order(qc))), qf[s], acc);
             s_acc[b] = acc;
         }
         if (masked) {
@@ -457,9 +502,8 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
             mx = fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, c));
         }
         const float m_new = fmaxf(m_run, mx * P.scale_log2e);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        if (__any(m_new > m_run)) {
-            const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+        if (__any(m_new > m_run + 8.0f)) {
+            const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
             l_run *= alpha;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -467,6 +511,7 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
                 for (int i = 0; i < 16; ++i) o_acc[b][i] *= alpha;
             m_run = m_new;
         }
+        const float m_use = m_run == -INFINITY ? 0.f : m_run;
         v8 pf[KS];
         float sum = 0.f;
 #pragma unroll
@@ -480,8 +525,9 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
         l_run += sum;
         // slot (h, j) of step ks is key 16 ks + 8 (j >> 2) + 4 h + (j & 3): the order the weights stand in
         auto v_frag = [&](int ks, int b) {
-            const T* a = bv + (16 * ks + 4 * h + ((lane & 15) >> 2)) * VSTR + 32 * b + (lane & 16) + 4 * (lane & 3);
-            const u32x2 lo = read_transposed(a), hi = read_transposed(a + 8 * VSTR);
+            const int r = 4 * h + ((lane & 15) >> 2), c = 4 * b + ((lane >> 3) & 2) + ((lane & 3) >> 1);      // order(16 ks + r) = order(r)
+            const T* a = bv + 16 * ks * D + 4 * (lane & 1);
+            const u32x2 lo = read_transposed(a + r * D + 8 * (c ^ v_order(r))), hi = read_transposed(a + (r + 8) * D + 8 * (c ^ v_order(r + 8)));
             return __builtin_bit_cast(v8, u32x4{lo[0], lo[1], hi[0], hi[1]});
         };
 #pragma unroll
@@ -508,16 +554,26 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
 
     if (k0 < k1) {
         pages(k0);
-        load(k0);
-        stage(k0, 0);
+        if constexpr (Q8) { load_codes(k0); stage_codes(k0, 0); }
+        else fetch(k0, 0);
     }
+#pragma unroll
+    for (int s = 0; s < QS; ++s) arrived(qf[s]);
     int cur = 0;
     for (int key0 = k0; key0 < k1; key0 += PAT_BK, cur ^= 1) {
+        if constexpr (!Q8) loads_done();
         __syncthreads();
         const int nxt = key0 + PAT_BK;
-        if (nxt < k1) load(nxt);
+        if constexpr (Q8) {
+            if (nxt < k1) load_codes(nxt);
+        } else {
+            if (key0 + PAT_BK - 1 > lim0) clean(key0, cur);
+            if (nxt < k1) fetch(nxt, cur ^ 1);
+        }
         if (key0 <= lim_hi) compute(key0, cur, key0 + PAT_BK - 1 > lim_lo);
-        if (nxt < k1) stage(nxt, cur ^ 1);
+        if constexpr (Q8) {
+            if (nxt < k1) stage_codes(nxt, cur ^ 1);
+        }
     }
 
     {
