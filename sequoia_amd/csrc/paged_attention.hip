@@ -397,16 +397,27 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     auto v_order = [](int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 2) << 1) | ((r >> 2) & 3); };
     const int lim0 = lim_of_row0 < k1 ? lim_of_row0 : k1 - 1;           // keys up to here are seen by every row of the workgroup
     const int lrow = lane / LPR, lcol = lane % LPR;
-    // a wave's rows of a pass lie in one 16-row block, so in one page: its entry is uniform, the rows one behind the other
+    // A wave's rows of a pass lie in one 16-row block, so in one page: its entry is uniform, the rows one behind the other.  Pages of
+    // a tile's length or more hold all passes' rows: one look-up a tile instead of one a pass (60 scalar instructions of a tile's
+    // 600 or so).
     constexpr int RPW = 64 / LPR;
+    const bool whole = P.map.shift >= 6;
     int pg[PASSES];
     auto pages = [&](int key0) {
+        pg[0] = page_entry(P.map, I.seq, (key0 + wave * RPW) >> P.map.shift);
+        if (!whole) {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) pg[i] = page_entry(P.map, I.seq, (key0 + i * RPP + wave * RPW) >> P.map.shift);
+            for (int i = 1; i < PASSES; ++i) pg[i] = page_entry(P.map, I.seq, (key0 + i * RPP + wave * RPW) >> P.map.shift);
+        }
     };
     auto rows_of = [&](int key0, size_t (&row)[PASSES]) {   // takes the entries, and asks for those of the next tile first: loads end in order
+        row[0] = stored_row(P, check_page(P.map, pg[0]), I.kvh, key0 + wave * RPW);
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) row[i] = stored_row(P, check_page(P.map, pg[i]), I.kvh, key0 + i * RPP + wave * RPW);
+        for (int i = 1; i < PASSES; ++i) row[i] = row[0] + i * RPP;
+        if (!whole) {
+#pragma unroll
+            for (int i = 1; i < PASSES; ++i) row[i] = stored_row(P, check_page(P.map, pg[i]), I.kvh, key0 + i * RPP + wave * RPW);
+        }
         pages(key0 + PAT_BK);
     };
     // values of V that are not finite, in a tile that some row does not see all of: staged as 0, and their rows noted
@@ -475,14 +486,24 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     };
     auto compute = [&](int key0, int which, bool masked) {
         const T *bk = (const T*)lds + which * BUF, *bv = bk + PAT_BK * D;
-        floatx16 s_acc[2];
+        __builtin_amdgcn_s_setprio(1);              // over the other workgroup's wave, which has its exponentials to do meanwhile
+        floatx16 s_acc[2] = {};
+        {
+            auto k_frag = [&](int b, int s) { return *(const v8*)(bk + (32 * b + qc) * D + 8 * ((2 * s + h) ^ k_order(qc))); };
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            floatx16 acc = {};
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int s = 0; s < QS; ++s) acc = mfma32<T>(*(const v8*)(bk + (32 * b + qc) * D + 8 * ((2 * s + h) ^ k_order(qc))), qf[s], acc);
-            s_acc[b] = acc;
+                for (int s = 0; s < QS; ++s) s_acc[b] = mfma32<T>(k_frag(b, s), qf[s], s_acc[b]);
+            // LDS reads run four products ahead: left alone, each is issued next to the product that waits for it
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * QS - 4; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
         }
+        __builtin_amdgcn_s_setprio(0);
         if (masked) {
             int seen = lim - key0 - 4 * h;          // opaque, or the 32 differences to it are kept in registers over the whole loop
             asm("" : "+v"(seen));
