@@ -631,35 +631,42 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     }
 }
 
-// Joins the parts of the key axis: one workgroup a (row, head), its waves take the parts in turn.
+// Joins the parts of the key axis: one workgroup a (row, head); each of its waves takes every fourth part, four of them in
+// flight at once.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_attention_join_kernel(PagedAttnParams P, int tile_rows) {
+    constexpr int E = D / 64, MAX = 4;                      // outputs a lane, parts a wave at a time
+    typedef float vecE __attribute__((ext_vector_type(E)));
     __shared__ float acc[4][D];
-    const int t = blockIdx.x / P.n_heads, head = blockIdx.x % P.n_heads, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int t = blockIdx.x / P.n_heads, head = blockIdx.x % P.n_heads, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const size_t step = (size_t)P.n_rows * P.n_heads, row = (size_t)t * P.n_heads + head;
+    const bool there = lane < P.n_splits;                   // loaded before it is known how many parts the row has
+    float m = there ? P.part_ml[(row + lane * step) * 2] : -INFINITY, l = there ? P.part_ml[(row + lane * step) * 2 + 1] : 0.f;
     const int seq = seq_of_row(P.cu_rows, P.n_seqs, t);
     if (seq >= P.n_seqs) return;
     const int first = P.cu_rows[seq], rows = (P.cu_rows[seq + 1] - first) * P.group, past = P.seq_lens[seq];
     const int r = (t - first) * P.group + head % P.group;
-    const int parts = (attn_tile_end(P, past, rows, r / tile_rows, tile_rows) + P.split_len - 1) / P.split_len;
-    if (parts <= 1) return;                         // written already
-    const size_t step = (size_t)P.n_rows * P.n_heads, row = (size_t)t * P.n_heads + head;
-    const bool mine = lane < parts;                 // at most 64 parts
-    const float m = mine ? P.part_ml[(row + lane * step) * 2] : -INFINITY, l = mine ? P.part_ml[(row + lane * step) * 2 + 1] : 0.f;
+    const int parts = __builtin_amdgcn_readfirstlane((attn_tile_end(P, past, rows, r / tile_rows, tile_rows) + P.split_len - 1) / P.split_len);
+    if (parts <= 1) return;                                 // written already
+    if (lane >= parts) { m = -INFINITY; l = 0.f; }
     const float top = wave_max_f32_dpp(m);
-    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);       // 0 in the lanes behind the last part
     const float sum = wave_sum_f32_dpp(l * f);
-    constexpr int E = D / 64;
-    float o[E];
+    vecE mine = {};
+    for (int s0 = wave; s0 < parts; s0 += 4 * MAX) {
+        vecE o[MAX];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int s = wave; s < parts; s += 4) {
-        const float fs = __shfl(f, s, 64);
-        const float* src = P.part_o + (row + s * step) * D + lane * E;
+        for (int i = 0; i < MAX; ++i) {
+            const int s = s0 + 4 * i < parts ? s0 + 4 * i : s0;                   // no branch: all of them are in flight
+            o[i] = *(const vecE*)(P.part_o + (row + s * step) * D + lane * E);
+        }
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += src[e] * fs;
+        for (int i = 0; i < MAX; ++i) {
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (s0 + 4 * i) & 63));
+            mine += o[i] * (s0 + 4 * i < parts ? w : 0.f);
+        }
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[wave][lane * E + e] = o[e];
+    *(vecE*)&acc[wave][lane * E] = mine;
     __syncthreads();
     for (int d = threadIdx.x; d < D; d += 256) {
         const float inv = sum != 0.f ? 1.0f / sum : 0.f;
