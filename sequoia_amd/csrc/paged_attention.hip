@@ -24,9 +24,11 @@ struct PagedAttnParams {
     int n_seqs, n_rows, n_heads, h_kv, group;
     float scale_log2e;
     int max_len;                           // no sequence's keys go further (host's bound: the parts cover it)
-    int n_tiles, n_splits, split_len;      // row tiles a (sequence, KV head), parts of the key axis, keys a part
-    float* part_o;                         // [n_splits][n_rows * n_heads][D]: unnormalised
-    float* part_ml;                        // [n_splits][n_rows * n_heads][2]: maximum (log2 units), sum
+    int n_tiles, n_splits, split_len;      // tiles: row tiles a (sequence, KV head), parts of the key axis, keys a part
+    int tile_rows, n_groups;               // rows: workgroups that share the keys of all units; 0: one a unit
+    float* part_o;                         // unnormalised sums.  tiles: [n_splits][n_rows * n_heads][D]; rows: [2 * n_groups][rows a tile][D]
+    float* part_ml;                        // [..][2]: maximum (log2 units), sum
+    int2* units;                           // rows: [n_seqs * h_kv] {place of the first part, parts}
 };
 
 template <typename T> __device__ __forceinline__ floatx4 mfma16(typename vec_of<T>::v8 a, typename vec_of<T>::v8 b, floatx4 c) {
@@ -112,233 +114,363 @@ __device__ __forceinline__ size_t stored_row(const PagedAttnParams& P, int page,
     return (((size_t)page * P.h_kv + kvh) << P.map.shift) + (key & ((1 << P.map.shift) - 1));
 }
 
-// Few rows (a decoding step, a drafted chunk): bound by the bytes of K and V.  Four waves walk the 32-key chunks of the
-// workgroup's part in turn, each with its own running softmax, and join through LDS.  A chunk is fetched as whole rows (16 bytes
-// a lane, next chunk in flight while this one is computed), staged in the wave's own LDS and read back as
-//   S^T = K Q^T    A = K rows, B = Q: a lane holds 8 scores of one query row, in the order the second product wants them
-//   O^T += V^T P^T A = V^T (transposing LDS reads), B = P^T straight from the registers S^T left behind.
+// Few rows (a decoding step, a drafted chunk): bound by the bytes of K and V.  Four waves walk the 32-key chunks of a unit -- a
+// (sequence, KV head) pair -- in turn, each with its own running softmax, and join through LDS.  Per chunk
+//   S^T = K Q^T    A = K, B = Q, both straight from memory: the order of the contraction is free, so a lane takes a quarter of its
+//                  row as it lies (element g D / 4 + 8 s + j for slot (s, g, j)); a lane then holds 8 scores of one query row, in
+//                  the order the second product wants them
+//   O^T += V^T P^T A = V^T by transposing reads of the wave's own LDS, where V was put as whole rows; B = P^T straight from the
+//                  registers S^T left behind.
+// The keys of all units, in order, are shared out evenly over the workgroups that fit the card, in steps of 128: a workgroup takes
+// the end of one unit, whole ones, and the beginning of another, and leaves the sums of the first and the last for the join;
+// whatever the lengths, all of them end together.  The next chunk's rows are asked for as soon as this one's have left their
+// registers, the next unit's while this one's waves join.
 #define PAD_NW 4
 #define PAD_BK 32
+#define PAD_STEP (PAD_NW * PAD_BK)
+
+// the packed rows of sequence b, their first row, stored rows and key end; offsets that name no rows: none
+struct Rows { int first, rows, past, end; };
+__device__ __forceinline__ Rows rows_of_seq(const PagedAttnParams& P, int b) {
+    Rows R;
+    R.first = P.cu_rows[b];
+    const int n = P.cu_rows[b + 1] - R.first;
+    R.past = P.seq_lens[b];
+    R.rows = R.first >= 0 && n > 0 && n <= P.n_rows - R.first ? n * P.group : 0;
+    R.end = R.rows ? attn_tile_end(P, R.past, R.rows, 0, P.tile_rows) : 0;
+    return R;
+}
+__device__ __forceinline__ int steps_of(int end) { return (end + PAD_STEP - 1) / PAD_STEP; }
+
+// By one wave: the sequence that step `group * per` of all belongs to (n_seqs: none), the step's place among the sequence's (KV
+// heads one behind the other), and per, the steps a workgroup.  The host has seen to it that all steps' number fits 31 bits.
+__device__ __forceinline__ int share(const PagedAttnParams& P, int group, int& per, int& place) {
+    const int lane = threadIdx.x & 63;
+    int mine = lane < P.n_seqs ? steps_of(rows_of_seq(P, lane).end) : 0;
+    uint32_t total = wave_sum_u32_dpp(mine);
+    for (int base = 64; base < P.n_seqs; base += 64)
+        total += wave_sum_u32_dpp(base + lane < P.n_seqs ? steps_of(rows_of_seq(P, base + lane).end) : 0);
+    const uint32_t all = total * (uint32_t)P.h_kv, even = (all + P.n_groups - 1) / (uint32_t)P.n_groups;
+    per = even > 2 ? (int)even : 2;                         // a part of fewer keys costs more to join than to walk
+    const uint32_t at = (uint32_t)group * (uint32_t)per;
+    if (at >= all) return P.n_seqs;
+    uint32_t before = 0;
+    for (int base = 0;; base += 64) {
+        if (base) mine = base + lane < P.n_seqs ? steps_of(rows_of_seq(P, base + lane).end) : 0;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int w = __shfl_up(upto, o, 64); if (lane >= o) upto += w; }
+        const uint64_t hit = __ballot((before + (uint32_t)upto) * (uint32_t)P.h_kv > at);
+        if (hit) {
+            const int j = __builtin_ctzll(hit);
+            before += __builtin_amdgcn_readlane(upto, j) - __builtin_amdgcn_readlane(mine, j);
+            place = (int)(at - before * (uint32_t)P.h_kv);
+            return base + j;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+}
+
 template <typename T, int D, bool Q8, int MT>
-__global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(PagedAttnParams P) {
+__global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 2) paged_attention_rows_kernel(PagedAttnParams P) {
     typedef typename vec_of<T>::v8 v8;
     typedef typename vec_of<T>::v4 v4;
-    constexpr int EPL = Q8 ? 16 : 8, LPR = D / EPL, RPP = 64 / LPR, PASSES = PAD_BK / RPP;   // elements a lane, lanes a row, rows a pass
+    constexpr int ESZ = Q8 ? 1 : 2, LPR = D * ESZ / 16, RPP = 64 / LPR, PASSES = PAD_BK / RPP;   // lanes a row of V, rows a pass
+    constexpr int KL = D * ESZ / 64;                // 16-byte loads of a lane's quarter of a row of K
     constexpr int DSTEPS = D / 32, NT = D / 16, ROWS = 16 * MT;
-    constexpr int KSTR = D + 8, VSTR = D + 16;      // 16-byte reads of 16 rows, 8-byte transposing reads of 8 rows: all banks once
-    constexpr int WAVE_BYTES = PAD_BK * (KSTR + VSTR) * 2, OSTR = D + 4;
+    constexpr int VSTR = D + 16;                    // 8-byte transposing reads of 8 rows: all banks once
+    constexpr int WAVE_BYTES = PAD_BK * VSTR * 2, OSTR = D + 4;
     constexpr int LDS_BYTES = PAD_NW * (WAVE_BYTES > ROWS * OSTR * 4 ? WAVE_BYTES : ROWS * OSTR * 4);
     __shared__ __attribute__((aligned(16))) unsigned char lds[LDS_BYTES];
     __shared__ float lds_ml[PAD_NW][ROWS][2];
-    AttnItem I;
-    if (!attn_item(P, ROWS, I)) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, qc = lane & 15, g = lane >> 4;
-    const int k0 = I.split * P.split_len, k1 = I.end < k0 + P.split_len ? I.end : k0 + P.split_len;
-    T* my_k = (T*)(lds + wave * WAVE_BYTES);
-    T* my_v = my_k + PAD_BK * KSTR;
-
-    v8 qf[MT][DSTEPS];
-    int lim[MT];                                    // last key this lane's query row sees
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        int r = I.row0 + 16 * mt + qc;
-        r = r < I.rows ? r : I.rows - 1;
-        const int token = r / P.group, head = I.kvh * P.group + r - token * P.group;
-        lim[mt] = I.past + token;
-        const T* qr = (const T*)P.q + head * P.q_head_stride + (size_t)(I.first + token) * P.q_row_stride + 8 * g;
-#pragma unroll
-        for (int s = 0; s < DSTEPS; ++s) qf[mt][s] = *(const v8*)(qr + 32 * s);
-    }
-    const int lim0 = I.past + I.row0 / P.group;     // keys up to here are seen by every row of the tile
-
-    float m_run[MT], l_run[MT];
-    floatx4 o_acc[MT][NT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        m_run[mt] = -INFINITY; l_run[mt] = 0.f;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) o_acc[mt][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
-
-    u32x4 kr[PASSES], vr[PASSES];
-    uint32_t ksr[PASSES], vsr[PASSES];
     const int lrow = lane / LPR, lcol = lane % LPR;
-    // entries of the pages that hold the two 16-row halves of a chunk
-    auto pages = [&](int key0, int& a, int& b) {
-        a = page_entry(P.map, I.seq, key0 >> P.map.shift);
-        b = page_entry(P.map, I.seq, (key0 + 16) >> P.map.shift);
-    };
-    auto load = [&](int key0, int ea, int eb) {
-        const size_t ra = stored_row(P, check_page(P.map, ea), I.kvh, key0), rb = stored_row(P, check_page(P.map, eb), I.kvh, key0 + 16);
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const size_t r = i * RPP < 16 ? ra + i * RPP : rb + (i * RPP - 16);         // scalar
-            const uint32_t at = lane * 16;                                              // rows lie one behind the other
-            kr[i] = *(const u32x4*)((const uint8_t*)P.k + r * (D * (Q8 ? 1 : 2)) + at);
-            vr[i] = *(const u32x4*)((const uint8_t*)P.v + r * (D * (Q8 ? 1 : 2)) + at);
-            if constexpr (Q8) { ksr[i] = (P.ks + r)[lrow]; vsr[i] = (P.vs + r)[lrow]; }
-        }
-    };
-    constexpr int STEP = PAD_NW * PAD_BK;
-    int key0 = k0 + wave * PAD_BK, ea = 0, eb = 0;
-    if (key0 < k1) {
-        int fa, fb;
-        pages(key0, fa, fb);
-        pages(key0 + STEP, ea, eb);
-        load(key0, fa, fb);
+    T* my_v = (T*)(lds + wave * WAVE_BYTES);
+
+    // ---- where it is: all of this in scalar registers, so that what branches on it is uniform ----
+    int seq, kvh, from = 0, left = 0x7fffffff, per = 0;     // from: the step of the unit to begin with; left: steps still to do
+    if (P.n_groups) {
+        int place = 0;
+        seq = __builtin_amdgcn_readfirstlane(share(P, blockIdx.x, per, place));
+        if (seq >= P.n_seqs) return;
+        left = per = __builtin_amdgcn_readfirstlane(per);
+        from = __builtin_amdgcn_readfirstlane(place);
+    } else {
+        seq = blockIdx.x / P.h_kv;
     }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int s = 0; s < DSTEPS; ++s) arrived(qf[mt][s]);
-    for (; key0 < k1; key0 += STEP) {
-        const bool tail = key0 + PAD_BK > k1;       // rows behind the end hold anything: their weights are 0, and so are they
-        const bool masked = tail || key0 + PAD_BK - 1 > lim0;
-        uint32_t hidden = 0;                        // rows of the chunk with values that were taken out
+    Rows R;
+    int steps, upto, k0, k1, lim0;
+    auto at_seq = [&]() {
+        const Rows r = rows_of_seq(P, seq);
+        R.first = __builtin_amdgcn_readfirstlane(r.first);
+        R.rows = __builtin_amdgcn_readfirstlane(r.rows < ROWS ? r.rows : ROWS);
+        R.past = __builtin_amdgcn_readfirstlane(r.past);
+        R.end = __builtin_amdgcn_readfirstlane(r.end);
+        steps = steps_of(R.end);
+        lim0 = R.past;                              // keys up to here are seen by every row
+    };
+    auto at_unit = [&]() {
+        upto = left < steps - from ? from + left : steps;
+        k0 = from * PAD_STEP;
+        k1 = R.end < upto * PAD_STEP ? R.end : upto * PAD_STEP;
+    };
+    at_seq();
+    if (P.n_groups) {
+        kvh = from / steps;
+        from -= kvh * steps;
+    } else {
+        kvh = blockIdx.x - seq * P.h_kv;
+        if (R.rows == 0) return;
+    }
+    at_unit();
+
+    // ---- loads ----
+    u32x4 kr[2][KL], vr[PASSES];
+    uint32_t ksr[2], vsr[PASSES];
+    size_t row[2];                                  // scalar: first rows of the chunk's halves
+    int ea = 0, eb = 0;                             // entries of the pages that hold the halves of the next chunk
+    v8 qf[MT][DSTEPS];
+    int lim[MT];                                    // last key this lane's query row sees, here
+    auto pages = [&](int key0, int& a, int& b) {
+        a = page_entry(P.map, seq, key0 >> P.map.shift);
+        b = page_entry(P.map, seq, (key0 + 16) >> P.map.shift);
+    };
+    auto take = [&](int key0, int a, int b) {
+        row[0] = stored_row(P, check_page(P.map, a), kvh, key0);
+        row[1] = stored_row(P, check_page(P.map, b), kvh, key0 + 16);
+    };
+    auto load_v = [&]() {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            const int rr = i * RPP + lrow;
-            bool bad = false;
-            if constexpr (Q8) {
-                v8 lo, hi;
-                e4m3_expand<T>(kr[i], e4m3_scale(ksr[i]), lo, hi);
-                *(v8*)(my_k + rr * KSTR + 16 * lcol) = lo;
-                *(v8*)(my_k + rr * KSTR + 16 * lcol + 8) = hi;
-                if (tail && key0 + rr >= k1) { vr[i] = u32x4{0, 0, 0, 0}; vsr[i] = 127; }
-                e4m3_expand<T>(vr[i], e4m3_scale(vsr[i]), lo, hi);
-                if (masked) bad = take_nonfinite<T>(lo) | take_nonfinite<T>(hi);
-                *(v8*)(my_v + rr * VSTR + 16 * lcol) = lo;
-                *(v8*)(my_v + rr * VSTR + 16 * lcol + 8) = hi;
-            } else {
-                *(u32x4*)(my_k + rr * KSTR + 8 * lcol) = kr[i];
-                if (tail && key0 + rr >= k1) vr[i] = u32x4{0, 0, 0, 0};
-                v8 w = __builtin_bit_cast(v8, vr[i]);
-                if (masked) bad = take_nonfinite<T>(w);
-                *(v8*)(my_v + rr * VSTR + 8 * lcol) = w;
-            }
-            if (masked) {
-                const uint64_t lanes = __ballot(bad);
-                if (lanes)
-                    for (int j = 0; j < RPP; ++j) hidden |= (uint32_t)(((lanes >> (j * LPR)) & ((1ull << LPR) - 1)) != 0) << (i * RPP + j);
-            }
+            const size_t r = i * RPP < 16 ? row[0] + i * RPP : row[1] + (i * RPP - 16);
+            vr[i] = *(const u32x4*)((const uint8_t*)P.v + r * (D * ESZ) + (uint32_t)lane * 16);      // rows lie one behind the other
+            if constexpr (Q8) vsr[i] = (P.vs + r)[lrow];
         }
-        if (key0 + STEP < k1) {                     // the entries of the chunk after the next come first: loads end in order
-            const int fa = ea, fb = eb;
-            pages(key0 + 2 * STEP, ea, eb);
-            load(key0 + STEP, fa, fb);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        floatx4 s_acc[MT][2];
+    };
+    auto load_k = [&]() {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            v8 kf[DSTEPS];
 #pragma unroll
-            for (int s = 0; s < DSTEPS; ++s) kf[s] = *(const v8*)(my_k + (16 * t + qc) * KSTR + 32 * s + 8 * g);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int s = 0; s < DSTEPS; ++s) acc = mfma16<T>(kf[s], qf[mt][s], acc);
-                s_acc[mt][t] = acc;
-            }
+            for (int i = 0; i < KL; ++i)
+                kr[t][i] = *(const u32x4*)((const uint8_t*)P.k + row[t] * (D * ESZ) + (uint32_t)(qc * (D * ESZ) + g * (D * ESZ / 4)) + 16 * i);
+            if constexpr (Q8) ksr[t] = (P.ks + row[t])[qc];
         }
-        v8 pf[MT];
+    };
+    auto load_q = [&]() {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            float sv[8], cmax = -INFINITY;
+            int r = 16 * mt + qc;
+            r = r < R.rows ? r : R.rows - 1;
+            const int token = r / P.group, head = kvh * P.group + r - token * P.group;
+            lim[mt] = R.past + token < k1 ? R.past + token : k1 - 1;
+            const T* qr = (const T*)P.q + head * P.q_head_stride + (size_t)(R.first + token) * P.q_row_stride + g * (D / 4);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sv[j] = s_acc[mt][j >> 2][j & 3] * P.scale_log2e;
-            if (masked) {
-                int seen = (lim[mt] < k1 ? lim[mt] : k1 - 1) - key0 - 4 * g;       // opaque: not eight differences kept over the loop
-                asm("" : "+v"(seen));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sv[j] = 16 * (j >> 2) + (j & 3) <= seen ? sv[j] : -INFINITY;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) cmax = fmaxf(cmax, sv[j]);
-            cmax = group4_max(cmax);
-            const float m_new = fmaxf(m_run[mt], cmax);
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;       // nothing seen so far
-            if (__any(m_new > m_run[mt])) {
-                const float alpha = __builtin_amdgcn_exp2f(m_run[mt] - m_use);
-                l_run[mt] *= alpha;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) o_acc[mt][nt] *= alpha;
-                m_run[mt] = m_new;
-            }
-            float psum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float p = __builtin_amdgcn_exp2f(sv[j] - m_use);
-                psum += p;
-                pf[mt][j] = (T)p;
-            }
-            l_run[mt] += psum;
+            for (int s = 0; s < DSTEPS; ++s) qf[mt][s] = *(const v8*)(qr + 8 * s);
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const T* a0 = my_v + (4 * g + (qc >> 2)) * VSTR + 16 * nt + 4 * (qc & 3);
-            const u32x2 lo = read_transposed(a0), hi = read_transposed(a0 + 16 * VSTR);
-            const v8 vf = __builtin_bit_cast(v8, u32x4{lo[0], lo[1], hi[0], hi[1]});
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) o_acc[mt][nt] = mfma16<T>(vf, pf[mt], o_acc[mt][nt]);
-        }
-        while (hidden) {                            // wave-uniform, and hardly ever entered
-            const int key = key0 + __builtin_ctz(hidden);
-            hidden &= hidden - 1;
-            const size_t row = stored_row(P, check_page(P.map, page_entry(P.map, I.seq, key >> P.map.shift)), I.kvh, key);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float x[4];
-                hidden4<T, D, Q8>(P, row, 16 * nt + 4 * g, x);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o_acc[mt][nt][j] += key <= lim[mt] ? x[j] : 0.f;
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
+    };
+    {
+        int fa, fb;
+        pages(k0 + wave * PAD_BK, fa, fb);
+        pages(k0 + wave * PAD_BK + PAD_STEP, ea, eb);
+        take(k0 + wave * PAD_BK, fa, fb);           // (a wave without a chunk here loads one all the same, in bounds)
+        load_v();
+        load_k();
+        load_q();
     }
 
-    // ---- join the waves -------------------------------------------------------------------------
-    __syncthreads();                                // everyone is done with the staging area
-    float* lds_o = (float*)lds;
+    for (bool first_unit = true;; first_unit = false) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const float l = group4_sum(l_run[mt]);
-        if (g == 0) { lds_ml[wave][16 * mt + qc][0] = m_run[mt]; lds_ml[wave][16 * mt + qc][1] = l; }
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) *(floatx4*)(lds_o + (wave * ROWS + 16 * mt + qc) * OSTR + 16 * nt + 4 * g) = o_acc[mt][nt];
-    }
-    __syncthreads();
-    for (int e = tid; e < ROWS * (D / 4); e += PAD_NW * 64) {
-        const int row = e / (D / 4), col = 4 * (e % (D / 4)), r = I.row0 + row;
-        if (r >= I.rows) break;                     // rows ascend with e
-        float m = -INFINITY, l = 0.f;
+            for (int s = 0; s < DSTEPS; ++s) arrived(qf[mt][s]);
+        float m_run[MT], l_run[MT];
+        floatx4 o_acc[MT][NT];
 #pragma unroll
-        for (int w = 0; w < PAD_NW; ++w) m = fmaxf(m, lds_ml[w][row][0]);
-        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int mt = 0; mt < MT; ++mt) {
+            m_run[mt] = -INFINITY; l_run[mt] = 0.f;
 #pragma unroll
-        for (int w = 0; w < PAD_NW; ++w) {
-            const float mw = lds_ml[w][row][0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
-            l += lds_ml[w][row][1] * f;
-            o += *(const floatx4*)(lds_o + (w * ROWS + row) * OSTR + col) * f;
+            for (int i = 0; i < NT; ++i) o_acc[mt][i] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
-        const int token = r / P.group, head = I.kvh * P.group + r - token * P.group;
-        if (I.n_parts <= 1) {
-            const float inv = l != 0.f ? 1.0f / l : 0.f;            // a row that sees nothing: zeros
-            v4 res;
+
+        for (int key0 = k0 + wave * PAD_BK; key0 < k1; key0 += PAD_STEP) {
+            const bool tail = key0 + PAD_BK > k1;   // rows behind the end hold anything: their weights are 0, and so are they
+            const bool masked = tail || key0 + PAD_BK - 1 > lim0, more = key0 + PAD_STEP < k1;
+            uint32_t hidden = 0;                    // rows of the chunk with values that were taken out
 #pragma unroll
-            for (int j = 0; j < 4; ++j) res[j] = (T)(o[j] * inv);
-            *(v4*)((T*)P.out + (size_t)(I.first + token) * P.out_stride + (size_t)head * D + col) = res;
-        } else {
-            const size_t pr = ((size_t)I.split * P.n_rows + I.first + token) * P.n_heads + head;
-            *(floatx4*)(P.part_o + pr * D + col) = o;
-            if (col == 0) { P.part_ml[pr * 2] = m; P.part_ml[pr * 2 + 1] = l; }
+            for (int i = 0; i < PASSES; ++i) {
+                const int rr = i * RPP + lrow;
+                bool bad = false;
+                if (tail && key0 + rr >= k1) { vr[i] = u32x4{0, 0, 0, 0}; if constexpr (Q8) vsr[i] = 127; }
+                if constexpr (Q8) {
+                    v8 lo, hi;
+                    e4m3_expand<T>(vr[i], e4m3_scale(vsr[i]), lo, hi);
+                    if (masked) bad = take_nonfinite<T>(lo) | take_nonfinite<T>(hi);
+                    *(v8*)(my_v + rr * VSTR + 16 * lcol) = lo;
+                    *(v8*)(my_v + rr * VSTR + 16 * lcol + 8) = hi;
+                } else {
+                    v8 w = __builtin_bit_cast(v8, vr[i]);
+                    if (masked) bad = take_nonfinite<T>(w);
+                    *(v8*)(my_v + rr * VSTR + 8 * lcol) = w;
+                }
+                if (masked) {
+                    const uint64_t lanes = __ballot(bad);
+                    if (lanes)
+                        for (int j = 0; j < RPP; ++j) hidden |= (uint32_t)(((lanes >> (j * LPR)) & ((1ull << LPR) - 1)) != 0) << (i * RPP + j);
+                }
+            }
+            if (more) {                             // the entries of the chunk after the next come first: loads end in order
+                const int fa = ea, fb = eb;
+                pages(key0 + 2 * PAD_STEP, ea, eb);
+                take(key0 + PAD_STEP, fa, fb);
+                load_v();
+            }
+            floatx4 s_acc[MT][2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                v8 kf[DSTEPS];
+                if constexpr (Q8) {
+#pragma unroll
+                    for (int i = 0; i < KL; ++i) e4m3_expand<T>(kr[t][i], e4m3_scale(ksr[t]), kf[2 * i], kf[2 * i + 1]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < KL; ++i) kf[i] = __builtin_bit_cast(v8, kr[t][i]);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < DSTEPS; ++s) acc = mfma16<T>(kf[s], qf[mt][s], acc);
+                    s_acc[mt][t] = acc;
+                }
+            }
+            if (more) load_k();
+            v8 pf[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                float sv[8], cmax = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sv[j] = s_acc[mt][j >> 2][j & 3] * P.scale_log2e;
+                if (masked) {
+                    int seen = lim[mt] - key0 - 4 * g;      // opaque: not eight differences kept over the loop
+                    asm("" : "+v"(seen));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sv[j] = 16 * (j >> 2) + (j & 3) <= seen ? sv[j] : -INFINITY;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) cmax = fmaxf(cmax, sv[j]);
+                cmax = group4_max(cmax);
+                const float m_new = fmaxf(m_run[mt], cmax);
+                const float m_use = m_new == -INFINITY ? 0.f : m_new;       // nothing seen so far
+                if (__any(m_new > m_run[mt])) {
+                    const float alpha = __builtin_amdgcn_exp2f(m_run[mt] - m_use);
+                    l_run[mt] *= alpha;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) o_acc[mt][nt] *= alpha;
+                    m_run[mt] = m_new;
+                }
+                float psum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float p = __builtin_amdgcn_exp2f(sv[j] - m_use);
+                    psum += p;
+                    pf[mt][j] = (T)p;
+                }
+                l_run[mt] += psum;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const T* a0 = my_v + (4 * g + (qc >> 2)) * VSTR + 16 * nt + 4 * (qc & 3);
+                const u32x2 lo = read_transposed(a0), hi = read_transposed(a0 + 16 * VSTR);
+                const v8 vf = __builtin_bit_cast(v8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) o_acc[mt][nt] = mfma16<T>(vf, pf[mt], o_acc[mt][nt]);
+            }
+            while (hidden) {                        // wave-uniform, and hardly ever entered
+                const int key = key0 + __builtin_ctz(hidden);
+                hidden &= hidden - 1;
+                const size_t at = stored_row(P, check_page(P.map, page_entry(P.map, seq, key >> P.map.shift)), kvh, key);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float x[4];
+                    hidden4<T, D, Q8>(P, at, 16 * nt + 4 * g, x);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o_acc[mt][nt][j] += key <= lim[mt] ? x[j] : 0.f;
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
         }
+
+        // ---- join the waves, with the next unit's first loads on their way ----
+        const bool whole = from == 0 && upto == steps;
+        const int done_rows = R.rows, done_first = R.first, done_head = kvh * P.group;
+        if (P.n_groups && from == 0 && tid == 0) {  // where the join finds the unit's parts
+            int2* const u = P.units + seq * P.h_kv + kvh;
+            *u = int2{(int)(2 * blockIdx.x + (first_unit ? 0 : 1)), whole ? 1 : 1 + (steps - upto + per - 1) / per};
+        }
+        left -= upto - from;
+        bool next = P.n_groups && left > 0;
+        if (next) {
+            from = 0;
+            if (++kvh == P.h_kv) {
+                kvh = 0;
+                do ++seq; while (seq < P.n_seqs && (at_seq(), steps == 0));
+                next = seq < P.n_seqs;
+            }
+        }
+        int fa = 0, fb = 0;
+        if (next) {
+            at_unit();
+            pages(k0 + wave * PAD_BK, fa, fb);
+            pages(k0 + wave * PAD_BK + PAD_STEP, ea, eb);
+        }
+        __syncthreads();                            // everyone is done with the staging area
+        float* lds_o = (float*)lds;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const float l = group4_sum(l_run[mt]);
+            if (g == 0) { lds_ml[wave][16 * mt + qc][0] = m_run[mt]; lds_ml[wave][16 * mt + qc][1] = l; }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) *(floatx4*)(lds_o + (wave * ROWS + 16 * mt + qc) * OSTR + 16 * nt + 4 * g) = o_acc[mt][nt];
+        }
+        __syncthreads();
+        if (next) {
+            take(k0 + wave * PAD_BK, fa, fb);
+            load_v();
+            load_k();
+            load_q();
+        }
+        for (int e = tid; e < ROWS * (D / 4); e += PAD_NW * 64) {
+            const int r = e / (D / 4), col = 4 * (e % (D / 4));
+            if (r >= done_rows) break;              // rows ascend with e
+            float m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < PAD_NW; ++w) m = fmaxf(m, lds_ml[w][r][0]);
+            floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < PAD_NW; ++w) {
+                const float mw = lds_ml[w][r][0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
+                l += lds_ml[w][r][1] * f;
+                o += *(const floatx4*)(lds_o + (w * ROWS + r) * OSTR + col) * f;
+            }
+            if (whole) {
+                const int token = r / P.group, head = done_head + r - token * P.group;
+                const float inv = l != 0.f ? 1.0f / l : 0.f;        // a row that sees nothing: zeros
+                v4 res;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) res[j] = (T)(o[j] * inv);
+                *(v4*)((T*)P.out + (size_t)(done_first + token) * P.out_stride + (size_t)head * D + col) = res;
+            } else {
+                const size_t pr = (size_t)(2 * blockIdx.x + (first_unit ? 0 : 1)) * ROWS + r;
+                *(floatx4*)(P.part_o + pr * D + col) = o;
+                if (col == 0) { P.part_ml[pr * 2] = m; P.part_ml[pr * 2 + 1] = l; }
+            }
+        }
+        if (!next) return;
+        __syncthreads();                            // the sums have been read: LDS is free again
     }
 }
 
@@ -674,29 +806,94 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(PagedAttnPara
     }
 }
 
-struct AttnPlan { int tile_rows, n_tiles, n_splits, split_len; };
+// Joins what the workgroups of paged_attention_rows_kernel left of a unit: NW waves a (row, head), each takes every NWth part, eight
+// of them in flight at once.  A unit's first part lies where the workgroup that began it said, the others at the first place of
+// the workgroups behind it.
+template <typename T, int D, int ROWS, int NW>
+__global__ void __launch_bounds__(256) paged_attention_join_rows_kernel(PagedAttnParams P) {
+    constexpr int E = D / 64, MAX = 8;                      // outputs a lane, parts a wave at a time
+    typedef float vecE __attribute__((ext_vector_type(E)));
+    __shared__ float acc[4][D], sums[4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * (4 / NW) + wave / NW;
+    const int w = wave % NW, t = (int)(item / P.n_heads), head = (int)(item % P.n_heads);
+    const int seq = t < P.n_rows ? __builtin_amdgcn_readfirstlane(seq_of_row(P.cu_rows, P.n_seqs, t)) : P.n_seqs;
+    if (seq >= P.n_seqs) return;                            // (NW > 1: the whole block's row)
+    const int first = P.cu_rows[seq], n = P.cu_rows[seq + 1] - first, r = (t - first) * P.group + head % P.group;
+    if (first < 0 || n > P.n_rows - first || r < 0 || r >= ROWS) return;       // rows that were left out
+    const int2 u = P.units[seq * P.h_kv + head / P.group];
+    const int parts = __builtin_amdgcn_readfirstlane(u.y), g0 = __builtin_amdgcn_readfirstlane(u.x);
+    if (parts <= 1) return;                                 // written already
+    auto slot = [&](int p) { return (size_t)(p ? (g0 & ~1) + 2 * p : g0) * ROWS + r; };
+    float top = -INFINITY;
+    for (int p = lane; p < parts; p += 64) top = fmaxf(top, P.part_ml[slot(p) * 2]);
+    vecE mine = {};
+    float sum = 0.f;
+    for (int p0 = w; p0 < parts; p0 += NW * MAX) {
+        vecE o[MAX];
+        float m[MAX], l[MAX];
+#pragma unroll
+        for (int i = 0; i < MAX; ++i) {
+            const size_t at = slot(p0 + NW * i < parts ? p0 + NW * i : p0);       // no branch: all of them are in flight
+            m[i] = P.part_ml[at * 2];
+            l[i] = P.part_ml[at * 2 + 1];
+            o[i] = *(const vecE*)(P.part_o + at * D + lane * E);
+        }
+        if (p0 == w) top = wave_max_f32_dpp(top);
+#pragma unroll
+        for (int i = 0; i < MAX; ++i) {
+            const float f = p0 + NW * i < parts && m[i] > -INFINITY ? __builtin_amdgcn_exp2f(m[i] - top) : 0.f;
+            mine += o[i] * f;
+            sum += l[i] * f;
+        }
+    }
+    if constexpr (NW > 1) {
+        *(vecE*)&acc[wave][lane * E] = mine;
+        if (lane == 0) sums[wave] = sum;
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int i = 1; i < NW; ++i) { mine += *(const vecE*)&acc[i][lane * E]; sum += sums[i]; }
+    }
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+    T* dst = (T*)P.out + (size_t)t * P.out_stride + (size_t)head * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[e] = (T)(mine[e] * inv);
+}
 
-static AttnPlan attn_plan(int n_seqs, int max_rows, int max_len, int n_heads, int h_kv) {
-    AttnPlan A;
-    const int rows = max_rows * (n_heads / h_kv);
-    A.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
-    A.n_tiles = (rows + A.tile_rows - 1) / A.tile_rows;
-    const int64_t base = (int64_t)n_seqs * h_kv * A.n_tiles;
-    int64_t want = (2048 + base - 1) / base;
+struct AttnPlan { int tile_rows, n_tiles, n_splits, split_len, n_groups; size_t parts, bytes; };
+
+static AttnPlan attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_heads, int h_kv, int d) {
+    AttnPlan A = {};
+    if (max_rows > n_rows) max_rows = n_rows;
+    const int64_t rows = (int64_t)max_rows * (n_heads / h_kv), units = (int64_t)n_seqs * h_kv;
+    A.n_tiles = A.n_splits = 1;
+    A.split_len = max_len;
+    if (rows <= 32) {
+        A.tile_rows = rows <= 16 ? 16 : 32;
+        // as many workgroups as fit the card (256 CUs; by registers and LDS), but none for fewer than 256 keys
+        const int64_t fit = 256 * 2, most = units * ((max_len + 255) / 256);
+        A.n_groups = max_len <= 256 ? 0 : (int)(fit < most ? fit : most);
+        A.parts = (size_t)2 * A.n_groups * A.tile_rows;
+        if (A.n_groups) A.bytes = A.parts * (d + 2) * sizeof(float) + units * sizeof(int2);
+        return A;
+    }
+    A.tile_rows = 128;
+    A.n_tiles = (int)((rows + 127) / 128);
+    // few tiles: the key axis is split for about 2048 workgroups, four rounds of the two that share a CU, in parts of 256 keys or more
+    int64_t want = (2048 + units * A.n_tiles - 1) / (units * A.n_tiles);
     want = want > 64 ? 64 : want;
     int64_t len = (max_len + want - 1) / want;
     len = len < 256 ? 256 : len;
     A.split_len = (int)((len + 127) / 128 * 128);
     A.n_splits = (max_len + A.split_len - 1) / A.split_len;
-    if (A.n_splits < 1) A.n_splits = 1;
+    if (A.n_splits > 1) A.bytes = (A.parts = (size_t)A.n_splits * n_rows * n_heads) * (d + 2) * sizeof(float);
     return A;
 }
 
 extern "C" size_t sq_paged_attention_workspace_bytes(int n_seqs, int n_rows, int max_rows, int max_len, int n_heads, int h_kv, int d) {
     if (n_seqs <= 0 || n_rows <= 0 || max_rows <= 0 || max_len <= 0 || n_heads <= 0 || h_kv <= 0 || n_heads % h_kv || d <= 0) return 0;
-    if (max_rows > n_rows) max_rows = n_rows;
-    const AttnPlan A = attn_plan(n_seqs, max_rows, max_len, n_heads, h_kv);
-    return A.n_splits > 1 ? (size_t)A.n_splits * n_rows * n_heads * (d + 2) * sizeof(float) : 0;
+    return attn_plan(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d).bytes;
 }
 
 extern "C" int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t q_row_stride, const void* k_pages, const void* v_pages,
@@ -714,32 +911,36 @@ extern "C" int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t 
     if (!q || !k_pages || !v_pages || !out || !d_page_table || !d_seq_lens || !d_cu_rows) return SQ_EINVAL;
     if ((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) || ((uintptr_t)out & 7) || ((q_head_stride | q_row_stride) & 7) || (out_stride & 3))
         return SQ_EINVAL;
-    if (max_rows > n_rows) max_rows = n_rows;
-    const AttnPlan A = attn_plan(n_seqs, max_rows, max_len, n_heads, h_kv);
-    const size_t need = sq_paged_attention_workspace_bytes(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d);
-    if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return SQ_EINVAL;
-    const int64_t grid = (int64_t)n_seqs * h_kv * A.n_tiles * A.n_splits, join = (int64_t)n_rows * n_heads;
-    if (grid > 0x7fffffff || join > 0x7fffffff) return SQ_EUNSUPPORTED;
+    const AttnPlan A = attn_plan(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d);
+    if (A.bytes && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < A.bytes)) return SQ_EINVAL;
+    const int64_t grid = A.n_groups ? A.n_groups : (int64_t)n_seqs * h_kv * A.n_tiles * A.n_splits, join = (int64_t)n_rows * n_heads;
+    if (grid > 0x7fffffff || join > 0x7fffffff || (int64_t)n_seqs * h_kv * (max_len / 128 + 1) > 0x7fffffff) return SQ_EUNSUPPORTED;
     PagedAttnParams P = {q, q_head_stride, q_row_stride, k_pages, v_pages, (const uint8_t*)k_scales, (const uint8_t*)v_scales, out, out_stride,
                          {d_page_table, table_width, n_pages, shift}, d_seq_lens, d_cu_rows, n_seqs, n_rows, n_heads, h_kv, n_heads / h_kv,
-                         scale * 1.4426950408889634f, max_len, A.n_tiles, A.n_splits, A.split_len, (float*)workspace,
-                         need ? (float*)workspace + (size_t)A.n_splits * n_rows * n_heads * d : nullptr};
+                         scale * 1.4426950408889634f, max_len, A.n_tiles, A.n_splits, A.split_len, A.tile_rows, A.n_groups,
+                         (float*)workspace, (float*)workspace + A.parts * d, (int2*)((float*)workspace + A.parts * (d + 2))};
     hipStream_t st = (hipStream_t)stream;
-#define SQ_A(TT, DD, QQ, MM) hipLaunchKernelGGL((paged_attention_rows_kernel<TT, DD, QQ, MM>), dim3((unsigned)grid), dim3(PAD_NW * 64), 0, st, P)
-#define SQ_AT(TT, DD, QQ) hipLaunchKernelGGL((paged_attention_tiles_kernel<TT, DD, QQ>), dim3((unsigned)grid), dim3(PAT_NW * 64), 0, st, P)
-#define SQ_AM(TT, DD, QQ) do { if (A.tile_rows == 16) SQ_A(TT, DD, QQ, 1); else if (A.tile_rows == 32) SQ_A(TT, DD, QQ, 2); else SQ_AT(TT, DD, QQ); } while (0)
-#define SQ_AD(TT, DD) do { if (k_scales) SQ_AM(TT, DD, true); else SQ_AM(TT, DD, false); } while (0)
-    if (dtype == SQ_DTYPE_F16) { if (d == 128) SQ_AD(half_t, 128); else SQ_AD(half_t, 64); }
-    else                       { if (d == 128) SQ_AD(bf16_t, 128); else SQ_AD(bf16_t, 64); }
-#undef SQ_AD
-#undef SQ_AM
-#undef SQ_AT
-#undef SQ_A
-    int rc = sq_check_launch();
-    if (rc != SQ_OK || A.n_splits <= 1) return rc;
-#define SQ_J(TT, DD) hipLaunchKernelGGL((paged_attention_join_kernel<TT, DD>), dim3((unsigned)join), dim3(256), 0, st, P, A.tile_rows)
-    if (dtype == SQ_DTYPE_F16) { if (d == 128) SQ_J(half_t, 128); else SQ_J(half_t, 64); }
-    else                       { if (d == 128) SQ_J(bf16_t, 128); else SQ_J(bf16_t, 64); }
-#undef SQ_J
+#define SQ_LAUNCH(K, G, ...) hipLaunchKernelGGL(K, dim3((unsigned)(G)), dim3(256), 0, st, __VA_ARGS__)
+#define SQ_KERNELS(TT, DD, QQ) do { \
+        if (A.tile_rows == 16) SQ_LAUNCH((paged_attention_rows_kernel<TT, DD, QQ, 1>), grid, P); \
+        else if (A.tile_rows == 32) SQ_LAUNCH((paged_attention_rows_kernel<TT, DD, QQ, 2>), grid, P); \
+        else SQ_LAUNCH((paged_attention_tiles_kernel<TT, DD, QQ>), grid, P); \
+    } while (0)
+    // the join of few rows gives each four waves (a part of the key axis each at a time), of many one
+#define SQ_JOIN_ROWS(TT, DD, RR) do { \
+        if (join < 1024) SQ_LAUNCH((paged_attention_join_rows_kernel<TT, DD, RR, 4>), join, P); \
+        else SQ_LAUNCH((paged_attention_join_rows_kernel<TT, DD, RR, 1>), (join + 3) / 4, P); \
+    } while (0)
+#define SQ_TYPES(TT, DD) do { \
+        if (k_scales) SQ_KERNELS(TT, DD, true); else SQ_KERNELS(TT, DD, false); \
+        if (A.n_groups) { if (A.tile_rows == 16) SQ_JOIN_ROWS(TT, DD, 16); else SQ_JOIN_ROWS(TT, DD, 32); } \
+        else if (A.n_splits > 1) SQ_LAUNCH((paged_attention_join_kernel<TT, DD>), join, P, A.tile_rows); \
+    } while (0)
+    if (dtype == SQ_DTYPE_F16) { if (d == 128) SQ_TYPES(half_t, 128); else SQ_TYPES(half_t, 64); }
+    else                       { if (d == 128) SQ_TYPES(bf16_t, 128); else SQ_TYPES(bf16_t, 64); }
+#undef SQ_TYPES
+#undef SQ_JOIN_ROWS
+#undef SQ_KERNELS
+#undef SQ_LAUNCH
     return sq_check_launch();
 }
