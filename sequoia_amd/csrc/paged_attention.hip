@@ -116,15 +116,16 @@ __device__ __forceinline__ size_t stored_row(const PagedAttnParams& P, int page,
 
 // Few rows (a decoding step, a drafted chunk): bound by the bytes of K and V.  Four waves walk the 32-key chunks of a unit -- a
 // (sequence, KV head) pair -- in turn, each with its own running softmax, and join through LDS.  Per chunk
-//   S^T = K Q^T    A = K, B = Q, both straight from memory: the order of the contraction is free, so a lane takes a quarter of its
-//                  row as it lies (element g D / 4 + 8 s + j for slot (s, g, j)); a lane then holds 8 scores of one query row, in
-//                  the order the second product wants them
-//   O^T += V^T P^T A = V^T by transposing reads of the wave's own LDS, where V was put as whole rows; B = P^T straight from the
-//                  registers S^T left behind.
+//   S^T = K Q^T    A = K rows, B = Q: a lane holds 8 scores of one query row, in the order the second product wants them
+//   O^T += V^T P^T A = V^T by transposing LDS reads, B = P^T straight from the registers S^T left behind.
+// Both come as whole rows, 16 bytes a lane, past the caches (nothing reads them again before much else has passed through), and
+// go through the wave's own LDS.  Measured with 48 sequences of 300-6000 e4m3 keys | 16 chunks of 1-7 drafted rows, fp16: cached
+// loads 72 | 52 us; K straight into its product's registers, a quarter of a row a lane, cached beside uncached V 66 | 48 us,
+// uncached 64 | 60 us; this 64 | 46 us.
 // The keys of all units, in order, are shared out evenly over the workgroups that fit the card, in steps of 128: a workgroup takes
 // the end of one unit, whole ones, and the beginning of another, and leaves the sums of the first and the last for the join;
 // whatever the lengths, all of them end together.  The next chunk's rows are asked for as soon as this one's have left their
-// registers, the next unit's while this one's waves join.
+// registers, the next unit's while this one's waves join.  (Two workgroups a CU: three read 10 % slower.)
 #define PAD_NW 4
 #define PAD_BK 32
 #define PAD_STEP (PAD_NW * PAD_BK)
@@ -172,20 +173,19 @@ __device__ __forceinline__ int share(const PagedAttnParams& P, int group, int& p
 }
 
 template <typename T, int D, bool Q8, int MT>
-__global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 2) paged_attention_rows_kernel(PagedAttnParams P) {
+__global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(PagedAttnParams P) {
     typedef typename vec_of<T>::v8 v8;
     typedef typename vec_of<T>::v4 v4;
-    constexpr int ESZ = Q8 ? 1 : 2, LPR = D * ESZ / 16, RPP = 64 / LPR, PASSES = PAD_BK / RPP;   // lanes a row of V, rows a pass
-    constexpr int KL = D * ESZ / 64;                // 16-byte loads of a lane's quarter of a row of K
+    constexpr int ESZ = Q8 ? 1 : 2, LPR = D * ESZ / 16, RPP = 64 / LPR, PASSES = PAD_BK / RPP;   // lanes a row, rows a pass
     constexpr int DSTEPS = D / 32, NT = D / 16, ROWS = 16 * MT;
-    constexpr int VSTR = D + 16;                    // 8-byte transposing reads of 8 rows: all banks once
-    constexpr int WAVE_BYTES = PAD_BK * VSTR * 2, OSTR = D + 4;
+    constexpr int KSTR = D + 8, VSTR = D + 16;      // 16-byte reads of 16 rows, 8-byte transposing reads of 8 rows: all banks once
+    constexpr int WAVE_BYTES = PAD_BK * (KSTR + VSTR) * 2, OSTR = D + 4;
     constexpr int LDS_BYTES = PAD_NW * (WAVE_BYTES > ROWS * OSTR * 4 ? WAVE_BYTES : ROWS * OSTR * 4);
     __shared__ __attribute__((aligned(16))) unsigned char lds[LDS_BYTES];
     __shared__ float lds_ml[PAD_NW][ROWS][2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, qc = lane & 15, g = lane >> 4;
     const int lrow = lane / LPR, lcol = lane % LPR;
-    T* my_v = (T*)(lds + wave * WAVE_BYTES);
+    T *my_k = (T*)(lds + wave * WAVE_BYTES), *my_v = my_k + PAD_BK * KSTR;
 
     // ---- where it is: all of this in scalar registers, so that what branches on it is uniform ----
     int seq, kvh, from = 0, left = 0x7fffffff, per = 0;     // from: the step of the unit to begin with; left: steps still to do
@@ -225,8 +225,8 @@ __global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 
     at_unit();
 
     // ---- loads ----
-    u32x4 kr[2][KL], vr[PASSES];
-    uint32_t ksr[2], vsr[PASSES];
+    u32x4 kr[PASSES], vr[PASSES];
+    uint32_t ksr[PASSES], vsr[PASSES];
     size_t row[2];                                  // scalar: first rows of the chunk's halves
     int ea = 0, eb = 0;                             // entries of the pages that hold the halves of the next chunk
     v8 qf[MT][DSTEPS];
@@ -239,21 +239,14 @@ __global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 
         row[0] = stored_row(P, check_page(P.map, a), kvh, key0);
         row[1] = stored_row(P, check_page(P.map, b), kvh, key0 + 16);
     };
-    auto load_v = [&]() {
+    auto load = [&]() {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const size_t r = i * RPP < 16 ? row[0] + i * RPP : row[1] + (i * RPP - 16);
-            vr[i] = *(const u32x4*)((const uint8_t*)P.v + r * (D * ESZ) + (uint32_t)lane * 16);      // rows lie one behind the other
-            if constexpr (Q8) vsr[i] = (P.vs + r)[lrow];
-        }
-    };
-    auto load_k = [&]() {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-            for (int i = 0; i < KL; ++i)
-                kr[t][i] = *(const u32x4*)((const uint8_t*)P.k + row[t] * (D * ESZ) + (uint32_t)(qc * (D * ESZ) + g * (D * ESZ / 4)) + 16 * i);
-            if constexpr (Q8) ksr[t] = (P.ks + row[t])[qc];
+            const uint32_t at = (uint32_t)lane * 16;                    // rows lie one behind the other
+            kr[i] = __builtin_nontemporal_load((const u32x4*)((const uint8_t*)P.k + r * (D * ESZ) + at));
+            vr[i] = __builtin_nontemporal_load((const u32x4*)((const uint8_t*)P.v + r * (D * ESZ) + at));
+            if constexpr (Q8) { ksr[i] = (P.ks + r)[lrow]; vsr[i] = (P.vs + r)[lrow]; }
         }
     };
     auto load_q = [&]() {
@@ -263,9 +256,9 @@ __global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 
             r = r < R.rows ? r : R.rows - 1;
             const int token = r / P.group, head = kvh * P.group + r - token * P.group;
             lim[mt] = R.past + token < k1 ? R.past + token : k1 - 1;
-            const T* qr = (const T*)P.q + head * P.q_head_stride + (size_t)(R.first + token) * P.q_row_stride + g * (D / 4);
+            const T* qr = (const T*)P.q + head * P.q_head_stride + (size_t)(R.first + token) * P.q_row_stride + 8 * g;
 #pragma unroll
-            for (int s = 0; s < DSTEPS; ++s) qf[mt][s] = *(const v8*)(qr + 8 * s);
+            for (int s = 0; s < DSTEPS; ++s) qf[mt][s] = *(const v8*)(qr + 32 * s);
         }
     };
     {
@@ -273,8 +266,7 @@ __global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 
         pages(k0 + wave * PAD_BK, fa, fb);
         pages(k0 + wave * PAD_BK + PAD_STEP, ea, eb);
         take(k0 + wave * PAD_BK, fa, fb);           // (a wave without a chunk here loads one all the same, in bounds)
-        load_v();
-        load_k();
+        load();
         load_q();
     }
 
@@ -303,11 +295,15 @@ __global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 
                 if (tail && key0 + rr >= k1) { vr[i] = u32x4{0, 0, 0, 0}; if constexpr (Q8) vsr[i] = 127; }
                 if constexpr (Q8) {
                     v8 lo, hi;
+                    e4m3_expand<T>(kr[i], e4m3_scale(ksr[i]), lo, hi);
+                    *(v8*)(my_k + rr * KSTR + 16 * lcol) = lo;
+                    *(v8*)(my_k + rr * KSTR + 16 * lcol + 8) = hi;
                     e4m3_expand<T>(vr[i], e4m3_scale(vsr[i]), lo, hi);
                     if (masked) bad = take_nonfinite<T>(lo) | take_nonfinite<T>(hi);
                     *(v8*)(my_v + rr * VSTR + 16 * lcol) = lo;
                     *(v8*)(my_v + rr * VSTR + 16 * lcol + 8) = hi;
                 } else {
+                    *(u32x4*)(my_k + rr * KSTR + 8 * lcol) = kr[i];
                     v8 w = __builtin_bit_cast(v8, vr[i]);
                     if (masked) bad = take_nonfinite<T>(w);
                     *(v8*)(my_v + rr * VSTR + 8 * lcol) = w;
@@ -322,19 +318,16 @@ __global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 
                 const int fa = ea, fb = eb;
                 pages(key0 + 2 * PAD_STEP, ea, eb);
                 take(key0 + PAD_STEP, fa, fb);
-                load_v();
+                load();
             }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
             floatx4 s_acc[MT][2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 v8 kf[DSTEPS];
-                if constexpr (Q8) {
 #pragma unroll
-                    for (int i = 0; i < KL; ++i) e4m3_expand<T>(kr[t][i], e4m3_scale(ksr[t]), kf[2 * i], kf[2 * i + 1]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < KL; ++i) kf[i] = __builtin_bit_cast(v8, kr[t][i]);
-                }
+                for (int s = 0; s < DSTEPS; ++s) kf[s] = *(const v8*)(my_k + (16 * t + qc) * KSTR + 32 * s + 8 * g);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     floatx4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -343,7 +336,6 @@ __global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 
                     s_acc[mt][t] = acc;
                 }
             }
-            if (more) load_k();
             v8 pf[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -439,8 +431,7 @@ __global__ void __launch_bounds__(PAD_NW * 64, MT == 1 && (Q8 || D == 64) ? 3 : 
         __syncthreads();
         if (next) {
             take(k0 + wave * PAD_BK, fa, fb);
-            load_v();
-            load_k();
+            load();
             load_q();
         }
         for (int e = tid; e < ROWS * (D / 4); e += PAD_NW * 64) {
