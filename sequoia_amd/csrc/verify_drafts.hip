@@ -19,8 +19,8 @@
 
 struct RowPart { float top; int first; double sum; };      // maximum, its first index, sum of exp((x - top) / T)
 struct RowTotal { double top, sum; int first; };
-// accepted tokens; whether a token is still to be drawn, and from two rows; their maxima and 1 / sum
-struct Decided { int k, draw, two; double p_top, p_inv, q_top, q_inv; };
+// accepted tokens; whether a token is still to be drawn, and from two rows; their maxima and sums
+struct Decided { int k, draw, two; double p_top, p_sum, q_top, q_sum; };
 
 struct VerifyDraftsParams {
     const void *target, *draft; int64_t ld_t, ld_d;
@@ -227,7 +227,8 @@ __device__ __forceinline__ RowTotal row_total(const Exp2& E, const VerifyDraftsP
     return RowTotal{top, z, f};
 }
 
-// p and max(p - q, 0) of 4 consecutive tokens
+// Of 4 consecutive tokens: p, and max(p - q, 0), each up to a factor of its own (the rows' sums are multiplied crosswise, not
+// divided by: a draw needs no scale)
 template <typename T>
 __device__ __forceinline__ void residual4(const Exp2& E, const VerifyDraftsParams& P, int b, int at0, const Decided& W, double c, int at, int hi,
                                           double (&p)[4], double (&r)[4]) {
@@ -236,10 +237,10 @@ __device__ __forceinline__ void residual4(const Exp2& E, const VerifyDraftsParam
     if (W.two) load_row((const T*)P.draft + (int64_t)(at0 + W.k) * P.ld_d, at, hi, y);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        p[j] = at + j < hi ? weight(E, (double)x[j], W.p_top, c) * W.p_inv : 0.0;
+        p[j] = at + j < hi ? weight(E, (double)x[j], W.p_top, c) : 0.0;
         r[j] = p[j];
         if (W.two) {
-            const double d = p[j] - (at + j < hi ? weight(E, (double)y[j], W.q_top, c) * W.q_inv : 0.0);
+            const double d = p[j] * W.q_sum - (at + j < hi ? weight(E, (double)y[j], W.q_top, c) * W.p_sum : 0.0);
             r[j] = d < 0.0 ? 0.0 : d;                        // NaN stays
         }
     }
@@ -248,12 +249,14 @@ __device__ __forceinline__ void residual4(const Exp2& E, const VerifyDraftsParam
 // running sums over the lanes
 __device__ __forceinline__ double wave_scan_f64(double v) {
     const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double w = __shfl_up(v, o, 64);
-        if (lane >= o) v += w;
-    }
-    return v;
+#define SQ_STEP(n) { const uint64_t b = __builtin_bit_cast(uint64_t, v);        /* row_shr: the lane n below, of the same 16 */ \
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, 0x110 + (n), 0xf, 0xf, true); \
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), 0x110 + (n), 0xf, 0xf, true); \
+        v += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo); }
+    SQ_STEP(1) SQ_STEP(2) SQ_STEP(4) SQ_STEP(8)
+#undef SQ_STEP
+    const double a = lane_f64(v, 15), b = a + lane_f64(v, 31), c = b + lane_f64(v, 47);
+    return v + (lane < 16 ? 0.0 : lane < 32 ? a : lane < 48 ? b : c);
 }
 
 // One workgroup a (sequence, part).  All of them judge the sequence's drafted tokens, VD_KEEP at a time (groups of lanes total the
@@ -300,7 +303,7 @@ __global__ void __launch_bounds__(VD_DRAW_THREADS) verify_drafts_walk_kernel(Ver
             bool ok = false;
             if (tok >= 0 && tok < P.vocab) {
                 if (greedy) ok = p.sum == 0.0 && p.first == tok;     // first: no index where nothing is above -inf
-                else ok = (double)u * (weight(E, (double)y, q.top, c) / q.sum) < weight(E, (double)x, p.top, c) / p.sum;
+                else ok = (double)u * weight(E, (double)y, q.top, c) * p.sum < weight(E, (double)x, p.top, c) * q.sum;
             }
             if (!ok) atomicMin(&s_reject, base + (int)threadIdx.x);  // a minimum: the order does not matter
         }
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(VD_DRAW_THREADS) verify_drafts_walk_kernel(Ver
     const int k = s_reject;
     const bool two = k < n && !greedy;
     const RowTotal p = s_tot[k - base], q = two ? s_tot[VD_KEEP + k - base] : RowTotal{0.0, 1.0, 0};
-    const Decided W{k, greedy ? 0 : 1, two ? 1 : 0, p.top, 1.0 / p.sum, q.top, 1.0 / q.sum};
+    const Decided W{k, greedy ? 0 : 1, two ? 1 : 0, p.top, p.sum, q.top, q.sum};
     if (part == 0 && threadIdx.x == 0) {
         P.accepted[b] = k;
         P.decided[b] = W;
