@@ -50,19 +50,15 @@ __device__ __forceinline__ int check_page(const PageMap& M, int entry) {
     return (unsigned)p < (unsigned)M.n_pages ? p : 0;
 }
 
-// the sequence that row `t` of a ragged batch belongs to (n_seqs: none), by one wave: cu_rows is ascending, so it is the number
-// of sequences that end at or before t.  64 ends a load instead of a search's chain of dependent ones.
+// The sequence that row `t` of a ragged batch belongs to (n_seqs: none), by one wave: the first that ends behind t.  64 ends a load
+// instead of a search's chain of dependent ones.
 __device__ __forceinline__ int seq_of_row(const int32_t* cu_rows, int n_seqs, int t) {
     const int lane = threadIdx.x & 63;
-    int seq = 0;
     for (int base = 0; base < n_seqs; base += 64) {
-        const int i = base + lane;
-        const bool done = i < n_seqs && cu_rows[i + 1] <= t;
-        const int n = __popcll(__ballot(done));
-        seq += n;
-        if (n < 64) break;
+        const uint64_t hit = __ballot(base + lane < n_seqs && cu_rows[base + lane + 1] > t);
+        if (hit) return base + __builtin_ctzll(hit);
     }
-    return seq;
+    return n_seqs;
 }
 
 // 16 codes -> 16 values of T, exact: v_cvt_scalef32 multiplies by the power of two while it widens

@@ -101,7 +101,7 @@ __device__ __forceinline__ bool attn_item(const PagedAttnParams& P, int tile_row
     I.first = __builtin_amdgcn_readfirstlane(P.cu_rows[I.seq]);        // scalar registers: what branches on these is uniform
     const int n = __builtin_amdgcn_readfirstlane(P.cu_rows[I.seq + 1]) - I.first;
     I.past = __builtin_amdgcn_readfirstlane(P.seq_lens[I.seq]);
-    if (I.first < 0 || I.first + n > P.n_rows) return false;
+    if (I.first < 0 || n <= 0 || n > P.n_rows - I.first) return false;      // no rows, or offsets that name none
     I.rows = n * P.group;
     I.row0 = tile * tile_rows;
     if (I.row0 >= I.rows) return false;
@@ -767,8 +767,10 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(PagedAttnPara
     float m = there ? P.part_ml[(row + lane * step) * 2] : -INFINITY, l = there ? P.part_ml[(row + lane * step) * 2 + 1] : 0.f;
     const int seq = seq_of_row(P.cu_rows, P.n_seqs, t);
     if (seq >= P.n_seqs) return;
-    const int first = P.cu_rows[seq], rows = (P.cu_rows[seq + 1] - first) * P.group, past = P.seq_lens[seq];
-    const int r = (t - first) * P.group + head % P.group;
+    const int first = P.cu_rows[seq], n = P.cu_rows[seq + 1] - first, past = P.seq_lens[seq];
+    if (first < 0 || t < first || n > P.n_rows - first) return;
+    const int rows = n * P.group, r = (t - first) * P.group + head % P.group;
+    if (r >= P.n_tiles * tile_rows) return;                 // rows that were left out
     const int parts = __builtin_amdgcn_readfirstlane((attn_tile_end(P, past, rows, r / tile_rows, tile_rows) + P.split_len - 1) / P.split_len);
     if (parts <= 1) return;                                 // written already
     if (lane >= parts) { m = -INFINITY; l = 0.f; }

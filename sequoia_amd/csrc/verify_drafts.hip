@@ -147,12 +147,11 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_stats_kernel(VerifyD
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) load_row(src, lo + i * (8 * VD_THREADS) + 8 * threadIdx.x, hi, x[i]);
     // target rows of sequence b end at cu[b + 1] + b + 1, draft rows at cu[b + 1]
-    int seq = 0;
-    for (int base = 0; base < P.n_seqs; base += 64) {
+    int seq = P.n_seqs;
+    for (int base = 0; base < P.n_seqs && seq == P.n_seqs; base += 64) {
         const int i = base + lane;
-        const int n = __popcll(__ballot(i < P.n_seqs && (is_t ? P.cu[i + 1] + i + 1 <= row : P.cu[i + 1] <= row - n_target)));
-        seq += n;
-        if (n < 64) break;
+        const uint64_t hit = __ballot(i < P.n_seqs && (is_t ? P.cu[i + 1] + i + 1 > row : P.cu[i + 1] > row - n_target));
+        if (hit) seq = base + __builtin_ctzll(hit);
     }
     if (seq >= P.n_seqs) return;                             // behind the last sequence
     const double c = log2e_over(P.temps ? P.temps[seq] : P.temp);

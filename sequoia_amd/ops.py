@@ -495,7 +495,7 @@ class HipOps:
                         v_scales=None):
         """Attention of a ragged batch's new tokens (written before by rope_kv_write_paged): row cu_rows[b] + i of q [H, n_rows, D]
         sees keys [0, seq_lens[b] + i] of sequence b; out [n_rows, H D].  max_rows / max_len: no sequence brings more rows / ends
-        behind more keys (defaults: n_rows, the table's whole width); they size the launch, and rows and keys beyond them are left
+        behind more keys (defaults and caps: n_rows, the table's whole width); they size the launch, and rows and keys beyond them are left
         out.  The default max_len costs workgroups that find nothing to do."""
         dev, dt = q.device, q.dtype
         _on_device(dev, k_pages, v_pages, out, page_table, seq_lens, cu_rows, k_scales, v_scales)
@@ -510,9 +510,9 @@ class HipOps:
         _index(seq_lens, torch.int32, n_seqs, "seq_lens")
         _index(cu_rows, torch.int32, n_seqs + 1, "cu_rows")
         max_rows = n_rows if max_rows is None else min(int(max_rows), n_rows)
-        max_len = width * page_size if max_len is None else int(max_len)
-        if max_rows < 0 or not 0 <= max_len <= width * page_size:
-            raise ValueError(f"max_rows {max_rows} / max_len {max_len}: the table holds {width * page_size} keys a sequence")
+        max_len = width * page_size if max_len is None else min(int(max_len), width * page_size)
+        if max_rows < 0 or max_len < 0:
+            raise ValueError(f"max_rows {max_rows} / max_len {max_len}: expected bounds >= 0")
         if not 0.0 < scale < float("inf"):
             raise ValueError(f"scale: expected a positive number, got {scale}")
         need = self.lib.sq_paged_attention_workspace_bytes(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d)

@@ -305,6 +305,73 @@ def test_attention(ops, heads, h_kv, d, page, past, new, behind, dtype, quantise
     check_attention(pool, q, again, past, new, d ** -0.5)
 
 
+LONG = [
+    # heads, h_kv, d, page, past, new: parts of one KV head's keys in hundreds of workgroups, in two row tiles, in the tiled kernel
+    (4, 1, 64, 64, [70001], [1]),
+    (2, 1, 128, 16, [20000, 3], [2, 1]),
+    (8, 1, 64, 32, [3000, 511], [3, 4]),
+    (8, 1, 128, 256, [9000], [6]),
+    (16, 2, 128, 64, [2047, 0, 600], [9, 20, 16]),
+]
+
+
+@pytest.mark.parametrize("dtype,quantised", [(torch.float16, True), (torch.bfloat16, False)])
+@pytest.mark.parametrize("heads,h_kv,d,page,past,new", LONG)
+def test_attention_over_many_parts(ops, heads, h_kv, d, page, past, new, dtype, quantised):
+    pool = Pool([p + n for p, n in zip(past, new)], h_kv, d, page, dtype, quantised, 22)
+    q = (1.5 * torch.randn((heads, sum(new), d), generator=torch.Generator().manual_seed(9))).to(dtype)
+    for bounds in (dict(max_rows=max(new), max_len=max(p + n for p, n in zip(past, new))), {}):
+        out = run_attention(ops, pool, q.to(DEV), past, new, d ** -0.5, **bounds)
+        check_attention(pool, q, out, past, new, d ** -0.5)
+
+
+@pytest.mark.parametrize("heads,h_kv,d,most", [(8, 8, 64, 2), (16, 2, 128, 1), (8, 1, 128, 4), (6, 2, 64, 30)])
+def test_attention_of_many_sequences(ops, heads, h_kv, d, most):
+    """More sequences than a wave has lanes, some without rows, lengths from nothing to many steps: every key is somebody's."""
+    import random
+    rng = random.Random(heads * d + most)
+    n = 150
+    new = [rng.choice((0, 0, 1, rng.randint(1, most))) for _ in range(n)]
+    past = [rng.choice((0, rng.randint(0, 40), rng.randint(0, 900))) for _ in range(n)]
+    new[0] = new[-1] = 0
+    dtype = torch.float16
+    pool = Pool([p + m for p, m in zip(past, new)], h_kv, d, 32, dtype, False, 23)
+    q = torch.randn((heads, sum(new) + 3, d), generator=torch.Generator().manual_seed(1)).to(dtype)
+    for bounds in (dict(max_rows=most, max_len=max(p + m for p, m in zip(past, new))), {}):
+        out = run_attention(ops, pool, q.to(DEV), past, new, d ** -0.5, 3, **bounds)
+        check_attention(pool, q, out, past, new, d ** -0.5)
+
+
+@pytest.mark.parametrize("heads,h_kv,most", [(4, 4, 1), (8, 1, 4), (4, 1, 40)])
+def test_attention_with_offsets_that_name_no_rows(ops, heads, h_kv, most):
+    """Offsets outside the batch, a sequence with more rows than max_rows: such rows are left out, the other sequences' results and
+    everything else stay what they are."""
+    d, page, dtype = 64, 16, torch.float16
+    past, new = [500, 300, 700], [most, most, most]
+    pool = Pool([p + n for p, n in zip(past, new)], h_kv, d, page, dtype, False, 24)
+    rows = sum(new)
+    q = torch.randn((heads, rows, d), generator=torch.Generator().manual_seed(2)).to(dtype)
+    good = run_attention(ops, pool, q.to(DEV), past, new, d ** -0.5, max_rows=most, max_len=740)
+    for offsets in ([0, most, 2 * most, 1 << 30], [-5, most, 2 * most, rows], [0, most, 2 * most, 2 * most - 1]):
+        out = torch.full((rows, heads * d), 3.0, dtype=dtype, device=DEV)
+        ops.paged_attention(q.to(DEV), pool.dev[0], pool.dev[1], out, pool.table.to(DEV), i32(past), i32(offsets), d ** -0.5, max_rows=most, max_len=740)
+        out = out.cpu()
+        for b in range(3):
+            mine = slice(b * most, (b + 1) * most)
+            if offsets[b] == b * most and offsets[b + 1] == (b + 1) * most:
+                worst = (out[mine].double() - good[mine].double()).abs().max()       # the shares differ, so the sums' order may
+                assert float(worst) <= 2.0 ** -8, (offsets, b)
+            else:
+                assert bool((out[mine] == 3.0).all()), (offsets, b)
+    if heads // h_kv * (most - 1) <= 32 and most > 1:
+        out = torch.full((rows, heads * d), 3.0, dtype=dtype, device=DEV)
+        ops.paged_attention(q.to(DEV), pool.dev[0], pool.dev[1], out, pool.table.to(DEV), i32(past), cu(new).to(DEV), d ** -0.5, max_rows=1, max_len=740)
+        got = out.cpu().view(rows, heads, d)
+        k, v = (R.stored(pool.pages[i], None, pool.table[0], torch.arange(501)) for i in (0, 1))
+        want, bound = R.attention(q[:, :1].double(), k, v, 500, d ** -0.5, dtype)
+        assert bool(((got[:1].double() - want).abs() <= bound).all())                 # the first row is there whatever the bound
+
+
 @pytest.mark.parametrize("past,new", [([5000], [1]), ([2500, 40], [17, 2]), ([900], [150])])
 def test_attention_sharp_and_flat_rows(ops, past, new):
     """Scores of hundreds (one key holds all the weight, maxima that rise late) and of 0 (every key the same weight)."""
@@ -458,6 +525,32 @@ def test_attention_replays_in_a_graph_with_other_lengths(ops, past, new, heads):
         eager = torch.zeros_like(out)
         ops.paged_attention(q, out=eager, seq_lens=lens, cu_rows=rows, scale=d ** -0.5, **kw, **bounds)
         assert torch.equal(out, eager) and bool(out.abs().sum() > 0)
+
+
+def test_two_graphs_at_once(ops):
+    """Two captured calls replayed on two streams: each graph has its own workspace."""
+    h_kv, d, page, dtype = 2, 64, 32, torch.float16
+    pools = [Pool([4001], h_kv, d, page, dtype, False, s) for s in (3, 4)]
+    qs = [torch.randn((8, 1, d), generator=torch.Generator().manual_seed(s)).to(dtype).to(DEV) for s in (3, 4)]
+    alone = [run_attention(ops, p, q, [4000], [1], d ** -0.5) for p, q in zip(pools, qs)]
+    kws, lens, rows = [p.kw() for p in pools], i32([4000]), i32([0, 1])
+    outs = [torch.zeros((1, 8 * d), dtype=dtype, device=DEV) for _ in range(2)]
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for q, o, kw in zip(qs, outs, kws):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.paged_attention(q, out=o, seq_lens=lens, cu_rows=rows, scale=d ** -0.5, **kw)
+        graphs.append(graph)
+    for _ in range(10):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o, a in zip(outs, alone):
+            assert torch.equal(o.cpu(), a)
 
 
 def test_two_streams_at_once(ops):
