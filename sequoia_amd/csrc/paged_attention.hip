@@ -873,11 +873,12 @@ static AttnPlan attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int
     }
     A.tile_rows = 128;
     A.n_tiles = (int)((rows + 127) / 128);
-    // few tiles: the key axis is split for about 2048 workgroups, four rounds of the two that share a CU, in parts of 256 keys or more
-    int64_t want = (2048 + units * A.n_tiles - 1) / (units * A.n_tiles);
+    // Few tiles: the key axis is split for one round of the two workgroups that share a CU, in parts of 512 keys or more.  Parts are
+    // dear here, 128 rows of fp32 sums each: with four rounds in parts of 256, 2048 rows of 32 heads took 157 us instead of 59.
+    int64_t want = (512 + units * A.n_tiles - 1) / (units * A.n_tiles);
     want = want > 64 ? 64 : want;
     int64_t len = (max_len + want - 1) / want;
-    len = len < 256 ? 256 : len;
+    len = len < 512 ? 512 : len;
     A.split_len = (int)((len + 127) / 128 * 128);
     A.n_splits = (max_len + A.split_len - 1) / A.split_len;
     if (A.n_splits > 1) A.bytes = (A.parts = (size_t)A.n_splits * n_rows * n_heads) * (d + 2) * sizeof(float);

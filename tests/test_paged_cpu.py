@@ -70,16 +70,25 @@ def test_c_entries_with_nothing_to_do():
     assert lib.sq_paged_attention_workspace_bytes(0, 1, 1, 1, 4, 2, 64) == 0 and lib.sq_verify_drafts_workspace_bytes(0, 0, 10) == 0
 
 
-def test_workspace_of_the_attention_covers_every_part():
-    """Whatever the sizes, the parts of the key axis cover max_len and there are at most 64 (one lane each joins them)."""
+def test_workspace_of_the_attention():
+    """Up to 32 packed rows a KV head: two places of 16 or 32 rows for each of at most 512 workgroups, and two numbers a unit.  More:
+    whole parts of the key axis, at most 64 (a lane each joins them), none of fewer than 512 keys."""
     lib = native.load()
     for n_seqs in (1, 3, 64, 1000):
         for max_len in (1, 255, 257, 5000, 131072, 2_000_000):
             for max_rows in (1, 7, 129, 4096):
                 for heads, kv in ((12, 12), (64, 8), (8, 1)):
-                    rows = max_rows * n_seqs
-                    parts, left = divmod(lib.sq_paged_attention_workspace_bytes(n_seqs, rows, max_rows, max_len, heads, kv, 128), rows * heads * 130 * 4)
-                    assert left == 0 and parts <= 64 and parts != 1
+                    rows, packed = max_rows * n_seqs, max_rows * heads // kv
+                    got = lib.sq_paged_attention_workspace_bytes(n_seqs, rows, max_rows, max_len, heads, kv, 128)
+                    if packed <= 32:
+                        if max_len <= 256:
+                            assert got == 0
+                            continue
+                        groups, left = divmod(got - n_seqs * kv * 8, 2 * (16 if packed <= 16 else 32) * 130 * 4)
+                        assert left == 0 and 1 <= groups <= 512 and groups <= n_seqs * kv * -(-max_len // 256)
+                    else:
+                        parts, left = divmod(got, rows * heads * 130 * 4)
+                        assert left == 0 and parts <= 64 and parts != 1 and (parts == 0 or max_len > 512 * (parts - 1))
 
 
 def test_front_end_refuses_host_tensors():
