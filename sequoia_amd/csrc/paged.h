@@ -32,6 +32,9 @@ __device__ __forceinline__ int page_of(const PageMap& M, int b, int i) {
     return (unsigned)p < (unsigned)M.n_pages ? p : -1;
 }
 
+// Workgroups of up to 256 threads that one launch takes: the threads of a grid dimension are counted in 32 bits
+#define PAGED_MAX_GRID 0xffffff
+
 static inline int page_shift(int page_size) {
     for (int s = 4; s <= 8; ++s)
         if (page_size == 1 << s) return s;

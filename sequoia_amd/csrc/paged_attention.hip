@@ -156,7 +156,7 @@ __device__ __forceinline__ int share(const PagedAttnParams& P, int group, int& p
     const uint32_t at = (uint32_t)group * (uint32_t)per;
     if (at >= all) return P.n_seqs;
     uint32_t before = 0;
-    for (int base = 0;; base += 64) {
+    for (int base = 0; base < P.n_seqs; base += 64) {
         if (base) mine = base + lane < P.n_seqs ? steps_of(rows_of_seq(P, base + lane).end) : 0;
         int upto = mine;
 #pragma unroll
@@ -170,6 +170,7 @@ __device__ __forceinline__ int share(const PagedAttnParams& P, int group, int& p
         }
         before += __builtin_amdgcn_readlane(upto, 63);
     }
+    return P.n_seqs;
 }
 
 template <typename T, int D, bool Q8, int MT>
@@ -473,6 +474,13 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
 //   O^T += V^T P^T V^T by transposing LDS reads; a lane's outputs belong to the same row: rescaling is lane-local, and skipped
 //                  while no maximum of the wave moves.
 // Two workgroups share a CU, so that one's exponentials run beside the other's products.
+// A row's maximum is replaced only when it grows by more than a factor of 2^8: weights then reach 256 instead of 1, with the same
+// relative rounding to the element type and the same fp32 sum; what is lost is that the largest weight is no longer exactly 1, one
+// more rounding of half a step.  16-bit rows go global -> LDS without registers; e4m3 rows through registers, which widen them.
+// 4096 rows of 64 heads behind 4001 stored ones, 8 KV heads of 128, bf16: 771 us, 1.05 PFLOP/s of the products that the mask leaves
+// (a large library product here: 1.26).  Of a wave's 2000 or so cycles a tile, 1024 are products; the exponentials and the
+// maximum's pass run beside the other wave's products only in part (a priority for one of the two changes nothing; three workgroups
+// a CU do not fit the registers).
 #define PAT_NW 4
 #define PAT_BK 64
 template <typename T, int D, bool Q8>
@@ -815,8 +823,10 @@ __global__ void __launch_bounds__(256) paged_attention_join_rows_kernel(PagedAtt
     const int first = P.cu_rows[seq], n = P.cu_rows[seq + 1] - first, r = (t - first) * P.group + head % P.group;
     if (first < 0 || n > P.n_rows - first || r < 0 || r >= ROWS) return;       // rows that were left out
     const int2 u = P.units[seq * P.h_kv + head / P.group];
-    const int parts = __builtin_amdgcn_readfirstlane(u.y), g0 = __builtin_amdgcn_readfirstlane(u.x);
-    if (parts <= 1) return;                                 // written already
+    // a unit without keys (a length below zero) has no parts, and nobody wrote its entry: its rows are zeros
+    const bool none = attn_tile_end(P, P.seq_lens[seq], n * P.group, 0, ROWS) == 0;
+    const int parts = __builtin_amdgcn_readfirstlane(none ? 0 : u.y), g0 = __builtin_amdgcn_readfirstlane(u.x);
+    if (parts == 1) return;                                 // written already
     auto slot = [&](int p) { return (size_t)(p ? (g0 & ~1) + 2 * p : g0) * ROWS + r; };
     float top = -INFINITY;
     for (int p = lane; p < parts; p += 64) top = fmaxf(top, P.part_ml[slot(p) * 2]);
@@ -908,7 +918,8 @@ extern "C" int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t 
     const AttnPlan A = attn_plan(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d);
     if (A.bytes && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < A.bytes)) return SQ_EINVAL;
     const int64_t grid = A.n_groups ? A.n_groups : (int64_t)n_seqs * h_kv * A.n_tiles * A.n_splits, join = (int64_t)n_rows * n_heads;
-    if (grid > 0x7fffffff || join > 0x7fffffff || (int64_t)n_seqs * h_kv * (max_len / 128 + 1) > 0x7fffffff) return SQ_EUNSUPPORTED;
+    if (grid > PAGED_MAX_GRID || join > PAGED_MAX_GRID || (int64_t)n_seqs * h_kv * (max_len / 128 + 1) > 0x7fffffff) return SQ_EUNSUPPORTED;
+    if (max_len > 1 << 30) return SQ_EUNSUPPORTED;          // keys are counted in 32 bits, some tiles past the end
     PagedAttnParams P = {q, q_head_stride, q_row_stride, k_pages, v_pages, (const uint8_t*)k_scales, (const uint8_t*)v_scales, out, out_stride,
                          {d_page_table, table_width, n_pages, shift}, d_seq_lens, d_cu_rows, n_seqs, n_rows, n_heads, h_kv, n_heads / h_kv,
                          scale * 1.4426950408889634f, max_len, A.n_tiles, A.n_splits, A.split_len, A.tile_rows, A.n_groups,

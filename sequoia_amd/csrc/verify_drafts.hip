@@ -10,6 +10,9 @@
 // and the token in it.  The first reads every logit once; the others touch two rows a sequence and are bound by latency.  (The
 // draw in the second launch's last workgroup of a sequence: every workgroup's release writes its XCD's L2 back, and the 21 us of
 // the two launches at 64 sequences of 32000 tokens became 28.)
+// One sequence of five drafted tokens, 32000 tokens, fp16: 17.6 us (4.4 + 5.7 + 7.8 of the launches, each a chain of loads).  64
+// sequences of 0-8: 38.8 us, 20 of it the first launch, bound by its 64-bit operations (5.3 cycles a wave's instruction here) and
+// not by the 5.2 TB/s that its bytes would allow; 24 sequences of 2-6 with 128261 tokens, bf16: 48.8 us.
 #include "paged.h"
 
 #define VD_THREADS 256
@@ -424,6 +427,7 @@ extern "C" int sq_verify_drafts(const void* target_logits, int64_t ld_target, co
                                 void* stream) {
     if (n_seqs < 0 || n_drafts < 0 || vocab <= 0) return SQ_EINVAL;
     if (dtype != SQ_DTYPE_F16 && dtype != SQ_DTYPE_BF16 && dtype != SQ_DTYPE_F32) return SQ_EUNSUPPORTED;
+    if (vocab > 1 << 30) return SQ_EUNSUPPORTED;            // tokens are counted in 32 bits, a part past the end
     if (n_seqs == 0) return SQ_OK;
     if (!target_logits || !d_cu_drafts || !d_u_next || !d_n_accepted || !d_next_tokens || ld_target < vocab) return SQ_EINVAL;
     if (n_drafts && (!draft_logits || !d_draft_tokens || !d_u_accept || ld_draft < vocab)) return SQ_EINVAL;
@@ -431,7 +435,7 @@ extern "C" int sq_verify_drafts(const void* target_logits, int64_t ld_target, co
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < sq_verify_drafts_workspace_bytes(n_seqs, n_drafts, vocab)) return SQ_EINVAL;
     const DraftLayout L = draft_layout(n_seqs, n_drafts, vocab);
     const int64_t rows = 2 * (int64_t)n_drafts + n_seqs;
-    if (rows * L.parts > 0x7fffffff || (int64_t)n_seqs * L.draw_parts > 0x7fffffff) return SQ_EUNSUPPORTED;
+    if (rows * L.parts > PAGED_MAX_GRID || (int64_t)n_seqs * L.draw_parts > PAGED_MAX_GRID / 2) return SQ_EUNSUPPORTED;
     char* ws = (char*)workspace;
     VerifyDraftsParams P = {target_logits, draft_logits, ld_target, ld_draft, d_draft_tokens, d_cu_drafts, d_u_accept, d_u_next, d_temperature,
                             temperature, d_n_accepted, d_next_tokens, n_seqs, n_drafts, vocab, L.parts, L.draw_parts, (RowPart*)ws,

@@ -45,7 +45,7 @@ def _on_device(dev, *tensors):
 
 
 def _index(t, dtype, n, name):
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.dim() != 1 or not t.is_contiguous() or t.shape[0] < n:
         raise ValueError(f"{name}: expected {n} contiguous entries, got {tuple(t.shape)}")
@@ -57,7 +57,7 @@ def _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dtype):
     if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError(f"k_pages / v_pages: expected [n_pages, H_kv, page_size, D] twice, got {tuple(shape)}, {tuple(v_pages.shape)}")
     want = dtype if k_scales is None else torch.float8_e4m3fn
-    if k_pages.dtype != want or v_pages.dtype != want:
+    if k_pages.dtype is not want or v_pages.dtype is not want:
         raise TypeError(f"k_pages / v_pages: expected {want}, got {k_pages.dtype}, {v_pages.dtype}")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("k_pages / v_pages: must be contiguous")
@@ -65,15 +65,16 @@ def _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dtype):
         raise ValueError("k_scales / v_scales: both or none")
     if k_scales is not None:
         for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
-            if t.dtype != torch.uint8:
+            if t.dtype is not torch.uint8:
                 raise TypeError(f"{name}: expected torch.uint8, got {t.dtype}")
             if t.shape != shape[:3] or not t.is_contiguous():
                 raise ValueError(f"{name}: expected {tuple(shape[:3])} contiguous, got {tuple(t.shape)}")
-    if page_table.dtype != torch.int32:
+    if page_table.dtype is not torch.int32:
         raise TypeError(f"page_table: expected torch.int32, got {page_table.dtype}")
-    if page_table.dim() != 2 or not page_table.is_contiguous():
-        raise ValueError(f"page_table: expected [sequences, pages] contiguous, got {tuple(page_table.shape)}")
-    return (*shape, *page_table.shape)
+    table = page_table.shape
+    if len(table) != 2 or not page_table.is_contiguous():
+        raise ValueError(f"page_table: expected [sequences, pages] contiguous, got {tuple(table)}")
+    return (*shape, *table)
 
 
 class HipOps:
@@ -495,8 +496,8 @@ class HipOps:
                         v_scales=None):
         """Attention of a ragged batch's new tokens (written before by rope_kv_write_paged): row cu_rows[b] + i of q [H, n_rows, D]
         sees keys [0, seq_lens[b] + i] of sequence b; out [n_rows, H D].  max_rows / max_len: no sequence brings more rows / ends
-        behind more keys (defaults and caps: n_rows, the table's whole width); they size the launch, and rows and keys beyond them are left
-        out.  The default max_len costs workgroups that find nothing to do."""
+        behind more keys (defaults and caps: n_rows, the table's whole width); they size the launch; keys beyond them are left out, rows
+        may be.  The default max_len costs workgroups that find nothing to do."""
         dev, dt = q.device, q.dtype
         _on_device(dev, k_pages, v_pages, out, page_table, seq_lens, cu_rows, k_scales, v_scales)
         if dt not in (torch.float16, torch.bfloat16) or out.dtype != dt:
@@ -519,7 +520,7 @@ class HipOps:
         # one buffer a call, from the stream-ordered allocator: two streams or two captured graphs never share it
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         self._launch(dev, self.lib.sq_paged_attention, "sq_paged_attention",
-                     (q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+                     (q.data_ptr(), q.stride(0) if n_heads > 1 else 0, q.stride(1) if n_rows > 1 else 0, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
                       out.data_ptr(), out.stride(0) if n_rows > 1 else n_heads * d, page_table.data_ptr(), width, n_pages, page_size,
                       seq_lens.data_ptr(), cu_rows.data_ptr(), n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d, float(scale),
                       _DTYPE_CODES[dt], _ptr(ws), need))

@@ -162,3 +162,15 @@ def test_layers_of_a_quantised_cache():
     one = c.layer(1)
     assert one["k_pages"].dtype == torch.float8_e4m3fn and one["k_scales"].dtype == torch.uint8 and one["k_scales"].shape == (6, 2, 16)
     assert cache(dtype=torch.bfloat16).layer(0)["k_scales"] is None
+
+
+@pytest.mark.parametrize("fn,bad", [
+    (write, dict(n_rows=1 << 24)),                                        # more workgroups than a launch takes
+    (read, dict(n_seqs=1 << 24)),
+    (attend, dict(n_rows=1 << 24, max_rows=1 << 24, wsb=1 << 62)),
+    (attend, dict(width=1 << 28, max_len=(1 << 30) + 1)),                 # keys past 30 bits
+    (verify, dict(vocab=(1 << 30) + 1, ldt=1 << 31, ldd=1 << 31, wsb=1 << 62)),
+    (verify, dict(n=1 << 23, wsb=1 << 62)),
+])
+def test_c_entries_refuse_what_a_launch_does_not_hold(fn, bad):
+    assert fn(native.load(), **bad) == native.SQ_EUNSUPPORTED

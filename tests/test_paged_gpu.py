@@ -372,6 +372,25 @@ def test_attention_with_offsets_that_name_no_rows(ops, heads, h_kv, most):
         assert bool(((got[:1].double() - want).abs() <= bound).all())                 # the first row is there whatever the bound
 
 
+@pytest.mark.parametrize("heads,h_kv,new", [(4, 4, 3), (8, 1, 2), (2, 2, 40)])
+def test_attention_of_a_length_below_zero(ops, heads, h_kv, new):
+    """Rows that see nothing are zeros, also where a whole sequence has no key and its neighbours are split."""
+    d, page, dtype = 64, 16, torch.float16
+    past, news = [700, 0, 600], [new] * 3
+    pool = Pool([p + n for p, n in zip(past, news)], h_kv, d, page, dtype, False, 25)
+    q = torch.randn((heads, 3 * new, d), generator=torch.Generator().manual_seed(3)).to(dtype)
+    for below in (1, new, new + 5, 1 << 30):
+        out = torch.full((3 * new, heads * d), 3.0, dtype=dtype, device=DEV)
+        ops.paged_attention(q.to(DEV), pool.dev[0], pool.dev[1], out, pool.table.to(DEV), i32([700, -below, 600]), cu(news).to(DEV), d ** -0.5,
+                            max_rows=new, max_len=740)
+        got = out.cpu()
+        assert bool((got[new:new + min(below, new)] == 0).all()), below
+        for b in (0, 2):
+            k, v = (R.stored(pool.pages[i], None, pool.table[b], torch.arange(past[b] + new)) for i in (0, 1))
+            want, bound = R.attention(q[:, b * new:(b + 1) * new].double(), k, v, past[b], d ** -0.5, dtype)
+            assert bool(((got[b * new:(b + 1) * new].view(new, heads, d).double() - want).abs() <= bound).all()), (below, b)
+
+
 @pytest.mark.parametrize("past,new", [([5000], [1]), ([2500, 40], [17, 2]), ([900], [150])])
 def test_attention_sharp_and_flat_rows(ops, past, new):
     """Scores of hundreds (one key holds all the weight, maxima that rise late) and of 0 (every key the same weight)."""
@@ -454,6 +473,15 @@ def test_attention_strided_queries_and_output(ops):
     ops.paged_attention(q, out=out[:, :heads * d], seq_lens=i32(past), cu_rows=cu(new).to(DEV), scale=d ** -0.5, **pool.kw())
     check_attention(pool, q.cpu(), out.cpu()[:, :heads * d], past, new, d ** -0.5)
     assert bool((out[:, heads * d:] == 3.0).all())
+
+
+def test_attention_of_one_row_and_one_head_of_any_strides(ops):
+    """A dimension of one element has no stride that matters."""
+    d, dtype = 64, torch.float16
+    pool = Pool([300], 1, d, 16, dtype, False, 27)
+    q = torch.randn((1, 1, d), generator=torch.Generator().manual_seed(5)).to(dtype)
+    odd = torch.empty(512, dtype=dtype, device=DEV).as_strided((1, 1, d), (3, 5, 1)).copy_(q)
+    check_attention(pool, q, run_attention(ops, pool, odd, [299], [1], d ** -0.5), [299], [1], d ** -0.5)
 
 
 def test_attention_and_write_in_a_cache_past_32_bit_offsets(ops):
