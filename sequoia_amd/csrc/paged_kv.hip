@@ -23,8 +23,8 @@ struct PagedWriteParams {
 // log2(D / 16) lane exchanges.  The products of two 16-bit values are exact in fp32; the one rounding of the sum is followed by
 // the one to the stored type.
 // Bound by bytes, read once and written once, and by latency below about a hundred rows: 6000 rows of 64 + 2 * 8 heads of 128, fp16,
-// 55.7 us (5.0 TB/s; a large copy here reaches 5.1); 32 rows into e4m3 pages 10.5 us a call, most of it the host's.  Stores past the
-// caches took 50.8 us, but the attention that follows reads these rows: kept cached.
+// 51 us (5.5 TB/s, a large copy here reaches 5.1); 32 rows into e4m3 pages 10.5 us a call, most of it the host's.  The stores go past
+// the caches: cached ones took 55.6 us, and the attention that reads the rows next, mostly on another XCD, takes the same time.
 template <typename T, int D, bool Q8>
 __global__ void __launch_bounds__(PKV_THREADS) rope_kv_write_paged_kernel(PagedWriteParams P) {
     typedef typename vec_of<T>::v8 v8;
@@ -56,8 +56,8 @@ __global__ void __launch_bounds__(PKV_THREADS) rope_kv_write_paged_kernel(PagedW
 #pragma unroll
         for (int j = 0; j < 8; ++j) { o1[j] = (T)x1[j]; o2[j] = (T)x2[j]; }
         T* dst = (T*)P.q_out + ((size_t)unit * P.n_rows + t) * D + 8 * c;
-        *(v8*)dst = o1;
-        *(v8*)(dst + D / 2) = o2;
+        __builtin_nontemporal_store(o1, (v8*)dst);
+        __builtin_nontemporal_store(o2, (v8*)(dst + D / 2));
     }
     const bool is_v = unit >= P.n_heads + P.h_kv;
     const int kvh = unit - P.n_heads - (is_v ? P.h_kv : 0);
@@ -70,8 +70,8 @@ __global__ void __launch_bounds__(PKV_THREADS) rope_kv_write_paged_kernel(PagedW
 #pragma unroll
         for (int j = 0; j < 8; ++j) { o1[j] = (T)x1[j]; o2[j] = (T)x2[j]; }
         T* dst = (T*)(is_v ? P.v : P.k) + r * D + 8 * c;
-        *(v8*)dst = o1;
-        *(v8*)(dst + D / 2) = o2;
+        __builtin_nontemporal_store(o1, (v8*)dst);
+        __builtin_nontemporal_store(o2, (v8*)(dst + D / 2));
     } else {
         // Magnitudes stop at the largest value of T that has four significant bits: one more step would read back as infinity.
         // An element that is not finite is stored as NaN and has no part in the scale.
@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(PKV_THREADS) rope_kv_write_paged_kernel(PagedW
             w2[h] = __builtin_amdgcn_cvt_pk_fp8_f32(y2[2], y2[3], __builtin_amdgcn_cvt_pk_fp8_f32(y2[0], y2[1], 0, false), true);
         }
         uint8_t* dst = (uint8_t*)(is_v ? P.v : P.k) + r * D + 8 * c;
-        *(u32x2*)dst = w1;
-        *(u32x2*)(dst + D / 2) = w2;
+        __builtin_nontemporal_store(w1, (u32x2*)dst);
+        __builtin_nontemporal_store(w2, (u32x2*)(dst + D / 2));
         if (c == 0) (is_v ? P.vs : P.ks)[r] = (uint8_t)x;
     }
 }
@@ -151,21 +151,26 @@ struct PagedReadParams {
     int n_blocks, h_kv;                 // workgroups over a sequence's rows
 };
 
-// One workgroup: PKV_READ_ROWS rows of one (sequence, KV head), K and V.  A lane moves 16 stored bytes of a row at a time, every
-// pass's loads issued before the first store.  Bound by bytes: eight sequences of 700-9000 e4m3 rows of 8 heads of 128 to bf16, 48 us
-// (4.4 TB/s: the workgroups of a short sequence behind its end still start, and look); one of 230 rows 9.3 us a call, the host's.
+// One workgroup: PKV_READ_ROWS rows of one (sequence, KV head), K and V.  A lane moves eight elements of a row at a time, so that
+// loads and stores both cover whole lines, every pass's loads issued before the first store; the rows go past the caches, other
+// layers' come before anybody reads them.  Bound by bytes: eight sequences of 700-9000 e4m3 rows of 8 heads of 128 to bf16, 33.6 us
+// (6.2 TB/s; cached stores 45; sixteen codes a lane, whose two stores leave every other 16 bytes to each other, 48; 64 rows a workgroup
+// 49, loads past the caches too 41).  One sequence of 230 rows: 9.3 us a call, the host's.
+template <bool Q8> struct stored8 { typedef u32x4 type; };
+template <> struct stored8<true> { typedef u32x2 type; };
 #define PKV_READ_ROWS 32
 template <typename T, int D, bool Q8>
 __global__ void __launch_bounds__(PKV_THREADS) kv_read_paged_kernel(PagedReadParams P) {
     typedef typename vec_of<T>::v8 v8;
-    constexpr int LPR = Q8 ? D / 16 : D / 8;                          // lanes a row
+    typedef typename stored8<Q8>::type piece;
+    constexpr int LPR = D / 8;                                        // lanes a row
     constexpr int RPP = PKV_THREADS / LPR;                            // rows a pass
     constexpr int PASSES = PKV_READ_ROWS > RPP ? PKV_READ_ROWS / RPP : 1;
     const int blk = blockIdx.x % P.n_blocks, bh = blockIdx.x / P.n_blocks, h = bh % P.h_kv, b = bh / P.h_kv;
     int n = P.counts[b];
     n = n < P.out_rows ? n : P.out_rows;
     const int first = blk * (PASSES * RPP) + threadIdx.x / LPR, c = threadIdx.x % LPR, start = P.starts[b];
-    u32x4 kr[PASSES], vr[PASSES];
+    piece kr[PASSES], vr[PASSES];
     uint32_t ks[PASSES], vs[PASSES];
     bool ok[PASSES];
 #pragma unroll
@@ -175,26 +180,26 @@ __global__ void __launch_bounds__(PKV_THREADS) kv_read_paged_kernel(PagedReadPar
         ok[i] = page >= 0;
         if (ok[i]) {
             const size_t r = (((size_t)page * P.h_kv + h) << P.map.shift) + (slot & ((1 << P.map.shift) - 1));
-            const size_t at = r * D * (Q8 ? 1 : 2) + 16 * c;
-            kr[i] = *(const u32x4*)((const uint8_t*)P.k + at);
-            vr[i] = *(const u32x4*)((const uint8_t*)P.v + at);
+            const size_t at = (r * D + 8 * c) * (Q8 ? 1 : 2);
+            kr[i] = *(const piece*)((const uint8_t*)P.k + at);
+            vr[i] = *(const piece*)((const uint8_t*)P.v + at);
             if constexpr (Q8) { ks[i] = P.ks[r]; vs[i] = P.vs[r]; }
         }
     }
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         if (!ok[i]) continue;
-        const size_t at = (size_t)b * P.seq_stride + (size_t)h * P.head_stride + (size_t)(first + i * RPP) * D + (Q8 ? 16 : 8) * c;
+        const size_t at = (size_t)b * P.seq_stride + (size_t)h * P.head_stride + (size_t)(first + i * RPP) * D + 8 * c;
         T *kd = (T*)P.k_out + at, *vd = (T*)P.v_out + at;
         if constexpr (Q8) {
             v8 lo, hi;
-            e4m3_expand<T>(kr[i], e4m3_scale(ks[i]), lo, hi);
-            *(v8*)kd = lo; *(v8*)(kd + 8) = hi;
-            e4m3_expand<T>(vr[i], e4m3_scale(vs[i]), lo, hi);
-            *(v8*)vd = lo; *(v8*)(vd + 8) = hi;
+            e4m3_expand<T>(u32x4{kr[i][0], kr[i][1], 0, 0}, e4m3_scale(ks[i]), lo, hi);
+            __builtin_nontemporal_store(lo, (v8*)kd);
+            e4m3_expand<T>(u32x4{vr[i][0], vr[i][1], 0, 0}, e4m3_scale(vs[i]), lo, hi);
+            __builtin_nontemporal_store(lo, (v8*)vd);
         } else {
-            *(u32x4*)kd = kr[i];
-            *(u32x4*)vd = vr[i];
+            __builtin_nontemporal_store(kr[i], (piece*)kd);
+            __builtin_nontemporal_store(vr[i], (piece*)vd);
         }
     }
 }
@@ -212,7 +217,7 @@ extern "C" int sq_kv_read_paged(const void* k_pages, const void* v_pages, const 
     if (!k_pages || !v_pages || !k_out || !v_out || !d_page_table || !d_starts || !d_counts) return SQ_EINVAL;
     if (((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return SQ_EINVAL;
     if (((out_seq_stride | out_head_stride) & 7) || out_head_stride < (int64_t)out_rows * d) return SQ_EINVAL;
-    const int rpp = PKV_THREADS / (k_scales ? d / 16 : d / 8), per = rpp > PKV_READ_ROWS ? rpp : PKV_READ_ROWS;
+    const int rpp = PKV_THREADS / (d / 8), per = rpp > PKV_READ_ROWS ? rpp : PKV_READ_ROWS;
     const int n_blocks = (max_count + per - 1) / per;
     const int64_t grid = (int64_t)n_blocks * h_kv * n_seqs;
     if (grid > PAGED_MAX_GRID) return SQ_EUNSUPPORTED;
