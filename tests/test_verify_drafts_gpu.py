@@ -182,3 +182,41 @@ def test_replays_in_a_graph(ops):
         torch.cuda.synchronize()
         want = run(ops, t, d, tok, cu, a.cpu(), u.cpu(), temps.cpu().tolist())
         assert (acc.tolist(), nxt.tolist()) == want
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("counts,vocab", [([2, 0], 270001), ([1, 2], 8), ([2], 9), ([3, 1], 15), ([1] * 130, 21), ([2, 1], 513), ([40], 9000)])
+def test_odd_and_very_wide_vocabularies(ops, counts, vocab, dtype):
+    """More than 64 parts of a row and 512 blocks of tokens; rows that end inside a lane's eight tokens; more sequences than a wave."""
+    check(ops, *case(counts, vocab, dtype, 3 * vocab + len(counts), masked=0.05), 0.9)
+
+
+@pytest.mark.parametrize("vocab", [3000, 32000, 140000])
+def test_a_long_chain_is_judged_to_its_end(ops, vocab):
+    """u = 0 accepts whatever has mass: all tokens of a chain that takes several steps, up to the one planted without any."""
+    counts = [70, 9, 33]
+    t, d, tok, cu, ua, un = case(counts, vocab, torch.bfloat16, 31)
+    ua.zero_()
+    assert check(ops, t, d, tok, cu, ua, un, 0.8)[0] == counts
+    t[66, tok[66]] = t[cu[2] + 2 + 32, tok[cu[2] + 32]] = -math.inf      # sequence 0's token 66, sequence 2's last
+    assert check(ops, t, d, tok, cu, ua, un, 0.8)[0] == [66, 9, 32]
+    check(ops, t, d, tok, cu, ua, un, 0.0)
+
+
+@pytest.mark.parametrize("vocab", [5000, 40000])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_rows_whose_maximum_comes_late(ops, vocab, dtype):
+    """The running maximum moves with every chunk of a row, by little and by so much that nothing before it counts; chunks and parts
+    that hold nothing."""
+    counts = [2] * 4
+    t, d, tok, cu, ua, un = case(counts, vocab, dtype, 41)
+    ramp = torch.linspace(-1.0, 1.0, vocab)
+    for b, height in enumerate((4.0, 900.0, -30000.0)):
+        t[3 * b:3 * b + 3] = (t[3 * b:3 * b + 3].float() * 0.2 + height * ramp).to(dtype)
+        d[2 * b:2 * b + 2] = (d[2 * b:2 * b + 2].float() * 0.2 + height * ramp).to(dtype)
+        tok[2 * b:2 * b + 2] = d[2 * b:2 * b + 2].float().argmax(-1)
+    t[9:, :vocab - 700] = -math.inf
+    d[6:, 100:] = -math.inf
+    tok[6:] = 50
+    check(ops, t, d, tok, cu, ua, un, 1.1)
+    check(ops, t, d, tok, cu, ua, un, 0.0)
