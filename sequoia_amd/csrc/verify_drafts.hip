@@ -10,8 +10,8 @@
 // the token in it.  The first reads every logit once; the others touch two rows a sequence and are bound by the latency of their
 // chains of loads, so that neither has a barrier.  (The draw in the second launch's last workgroup of a sequence: every workgroup's
 // release writes its XCD's L2 back, and the two launches' time grew by a third.)
-// One sequence of five drafted tokens, 32000 tokens, fp16: 11.5 us on the device (3.4 + 4.6 + 3.5).  64 sequences of 0-8: 33 us, 20
-// of it the first launch, bound by the vector ALU -- 23 instructions a logit, of which 16 are 64-bit; every one of them takes four
+// One sequence of five drafted tokens, 32000 tokens, fp16: 11.8 us on the device.  64 sequences of 0-8: 31.5 us, 19 of it the first
+// launch, bound by the vector ALU -- 20 instructions a logit, of which 16 are 64-bit; every one of them takes four
 // cycles and a little, 64-bit or not -- and not by the 5.1 TB/s that its bytes would allow.  24 sequences of 2-6 with 128261 tokens,
 // bf16: 42 us, 28 of it the first launch.
 #include "paged.h"
@@ -157,13 +157,19 @@ __device__ __forceinline__ double wave_sum_f64(double v) {                      
     return (lane_f64(v, 0) + lane_f64(v, 16)) + (lane_f64(v, 32) + lane_f64(v, 48));
 }
 
+// (fmaxf() would first make every bf16 value canonical)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 // a uniform element, by the scalar unit: its wait is not one for the vector loads in flight
 template <typename V> __device__ __forceinline__ V scalar_load(const V* p) {
     return *(const __attribute__((address_space(4))) V*)(uintptr_t)p;
 }
 
 template <typename T, int CHUNKS, bool SHORT>
-__global__ void __launch_bounds__(VD_THREADS, 4) verify_drafts_stats_kernel(VerifyDraftsParams P) {
+__global__ void __launch_bounds__(VD_THREADS, 6) verify_drafts_stats_kernel(VerifyDraftsParams P) {
     constexpr int PART = 8 * CHUNKS * VD_THREADS;
     __shared__ float s_max[4];
     __shared__ int s_first;
@@ -220,25 +226,24 @@ __global__ void __launch_bounds__(VD_THREADS, 4) verify_drafts_stats_kernel(Veri
         float x[8];
         row8[i].behind(sum);
         values(i, x);
-        float m = x[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) m = fmaxf(m, x[j]);
+        float m = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
 #pragma unroll
         for (int j = 0; j < 8; j += 2) nan |= __builtin_isunordered(x[j], x[j + 1]);
-        m = wave_max_f32_dpp(m);
         if (c > 0.0) {
-            if (m > top) {
+            if (__any(m > top)) {                            // (seldom, after a row's first chunks)
+                m = wave_max_f32_dpp(m);
                 if (top > -INFINITY) sum *= weight(E, (double)top, (double)m, c);
                 shift = -(double)m * c;
+                top = m;
             }
-            if (fmaxf(m, top) > -INFINITY) sum += weights_in_sum(E, x, shift, c);       // else nothing so far counts
+            if (top > -INFINITY) sum += weights_in_sum(E, x, shift, c);       // else nothing so far counts
         } else {                                             // greedy: the first maximum
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (x[j] > best) { best = x[j]; first = row8[i].from + j; }
         }
-        top = fmaxf(m, top);
     }
+    if (c == 0.0) top = wave_max_f32_dpp(best);
     nan |= top == INFINITY;                                  // such a row is no distribution either
     sum = wave_sum_f64(nan ? NAN : sum);
     if (threadIdx.x == 0) s_first = 0x7fffffff;
@@ -477,9 +482,9 @@ __global__ void __launch_bounds__(64) verify_drafts_draw_kernel(VerifyDraftsPara
 }
 
 // Parts of 4096 tokens where the workgroups fit the card at once (8 a CU): a workgroup lives 3 us, most of it waiting for its loads.
-// Beyond that parts of 16384, whose chunks are summed while the later ones come: fewer sums a row to join, and the same time
-// (64 sequences of 32000 tokens: 20 us either way, 24 of 128261: 28.6 instead of 30.5).
-static int stats_part(int64_t rows, int vocab) { return rows * ((vocab - 1) / 4096 + 1) > 2048 ? 16384 : 4096; }
+// Beyond that parts of 8192, whose chunks are summed while the later ones come.  4096 | 8192 | 16384, 64 sequences of 32000 tokens:
+// 19.4 | 18.8 | 20.2 us, 24 of 128261: 30.2 | 28.7 | 28.0.
+static int stats_part(int64_t rows, int vocab) { return rows * ((vocab - 1) / 4096 + 1) > 2048 ? 8192 : 4096; }
 
 struct DraftLayout { size_t mass, decided, token_logit, bytes; int part, parts, blocks; };
 static DraftLayout draft_layout(int n_seqs, int n_drafts, int vocab) {
@@ -525,7 +530,7 @@ extern "C" int sq_verify_drafts(const void* target_logits, int64_t ld_target, co
     hipStream_t st = (hipStream_t)stream;
 #define SQ_V(TT, SS) do { \
         if (L.part == 4096) hipLaunchKernelGGL((verify_drafts_stats_kernel<TT, 2, SS>), dim3((unsigned)(rows * L.parts)), dim3(VD_THREADS), 0, st, P); \
-        else hipLaunchKernelGGL((verify_drafts_stats_kernel<TT, 8, SS>), dim3((unsigned)(rows * L.parts)), dim3(VD_THREADS), 0, st, P); \
+        else hipLaunchKernelGGL((verify_drafts_stats_kernel<TT, 4, SS>), dim3((unsigned)(rows * L.parts)), dim3(VD_THREADS), 0, st, P); \
         hipLaunchKernelGGL((verify_drafts_walk_kernel<TT, SS>), dim3((unsigned)walk), dim3(VD_THREADS), 0, st, P); \
         hipLaunchKernelGGL((verify_drafts_draw_kernel<TT, SS>), dim3((unsigned)n_seqs), dim3(64), 0, st, P); \
     } while (0)
