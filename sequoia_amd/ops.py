@@ -9,6 +9,8 @@ oracle/ops_adapter.py) to exercise the *host logic* on CPU; nothing in this pack
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import native
@@ -39,8 +41,9 @@ def _on_device(dev, *tensors):
     """Every tensor (None is allowed) on the device `dev` of the call: the launch goes to that device's current stream."""
     if dev.type != "cuda":
         raise native.SequoiaNativeError(f"the tensors live on {dev}: the paged path only runs on a HIP device (no CPU fallback)")
+    index = dev.index
     for t in tensors:
-        if t is not None and t.get_device() != dev.index:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"the call's tensors live on different devices: {[str(x.device) for x in tensors if x is not None]} beside {dev}")
 
 
@@ -82,6 +85,9 @@ class HipOps:
 
     def __init__(self):
         self.lib = native.load()
+        # sizes of sizes: the layers of a step ask for the same
+        self._attention_workspace = functools.lru_cache(256)(self.lib.sq_paged_attention_workspace_bytes)
+        self._verify_workspace = functools.lru_cache(256)(self.lib.sq_verify_drafts_workspace_bytes)
 
     @staticmethod
     def _stream():
@@ -426,11 +432,12 @@ class HipOps:
     def _launch(dev, fn, what, args):
         """fn(*args, stream) on `dev`'s current stream, with `dev` current for the launch."""
         # the raw handle: torch.cuda.current_stream() builds a Stream object, 2.7 us of a small call's 13
-        if dev.index == torch.cuda.current_device():
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        index = dev.index
+        if index == torch._C._cuda_getDevice():
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         else:
             with torch.cuda.device(dev):
-                rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         if rc:
             check(rc, what)
 
@@ -516,7 +523,7 @@ class HipOps:
             raise ValueError(f"max_rows {max_rows} / max_len {max_len}: expected bounds >= 0")
         if not 0.0 < scale < float("inf"):
             raise ValueError(f"scale: expected a positive number, got {scale}")
-        need = self.lib.sq_paged_attention_workspace_bytes(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d)
+        need = self._attention_workspace(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d)
         # one buffer a call, from the stream-ordered allocator: two streams or two captured graphs never share it
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         self._launch(dev, self.lib.sq_paged_attention, "sq_paged_attention",
@@ -556,7 +563,7 @@ class HipOps:
             _index(temps, torch.float32, n_seqs, "temperature")
         elif not 0.0 <= temperature < float("inf"):
             raise ValueError(f"temperature: expected a number >= 0, got {temperature}")
-        need = self.lib.sq_verify_drafts_workspace_bytes(n_seqs, n_drafts, vocab)
+        need = self._verify_workspace(n_seqs, n_drafts, vocab)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         self._launch(dev, self.lib.sq_verify_drafts, "sq_verify_drafts",
                      (target_logits.data_ptr(), max(target_logits.stride(0), vocab), _ptr(draft_logits) or None,
