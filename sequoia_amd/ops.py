@@ -50,8 +50,9 @@ def _on_device(dev, *tensors):
 def _index(t, dtype, n, name):
     if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.dim() != 1 or not t.is_contiguous() or t.shape[0] < n:
-        raise ValueError(f"{name}: expected {n} contiguous entries, got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 1 or shape[0] < n or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous entries, got {tuple(shape)}")
 
 
 def _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dtype):
@@ -449,26 +450,27 @@ class HipOps:
         Rows behind cu_rows[-1] are left alone."""
         dev, dt = qkv.device, qkv.dtype
         _on_device(dev, q_out, k_pages, v_pages, cos, sin, position_ids, page_table, seq_lens, cu_rows, k_scales, v_scales)
-        if dt not in (torch.float16, torch.bfloat16):
+        if dt is not torch.float16 and dt is not torch.bfloat16:
             raise TypeError(f"qkv: expected torch.float16 or torch.bfloat16, got {dt}")
-        for t, name in ((q_out, "q_out"), (cos, "cos"), (sin, "sin")):
-            if t.dtype != dt:
-                raise TypeError(f"{name}: expected {dt}, got {t.dtype}")
+        if q_out.dtype is not dt or cos.dtype is not dt or sin.dtype is not dt:
+            raise TypeError(f"q_out / cos / sin: expected {dt} three times, got {q_out.dtype}, {cos.dtype}, {sin.dtype}")
         n_pages, hk, page_size, dim, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
-        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (n_heads + 2 * h_kv) * d or (hk, dim) != (h_kv, d):
-            raise ValueError(f"qkv: expected [n_rows, {(n_heads + 2 * h_kv) * d}] with unit inner stride over pages of {h_kv} heads of {d}, "
-                             f"got {tuple(qkv.shape)} over {hk} heads of {dim}")
-        n_rows = qkv.shape[0]
+        shape, stride, cols = qkv.shape, qkv.stride(), (n_heads + 2 * h_kv) * d
+        if len(shape) != 2 or stride[1] != 1 or shape[1] != cols or hk != h_kv or dim != d:
+            raise ValueError(f"qkv: expected [n_rows, {cols}] with unit inner stride over pages of {h_kv} heads of {d}, "
+                             f"got {tuple(shape)} over {hk} heads of {dim}")
+        n_rows = shape[0]
         if q_out.shape != (n_heads, n_rows, d) or not q_out.is_contiguous():
             raise ValueError(f"q_out: expected {(n_heads, n_rows, d)} contiguous, got {tuple(q_out.shape)}")
-        if cos.dim() != 2 or cos.shape[1] != d or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
-            raise ValueError(f"cos / sin: expected [positions, {d}] contiguous twice, got {tuple(cos.shape)}, {tuple(sin.shape)}")
+        table = cos.shape
+        if len(table) != 2 or table[1] != d or table != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError(f"cos / sin: expected [positions, {d}] contiguous twice, got {tuple(table)}, {tuple(sin.shape)}")
         _index(position_ids, torch.int64, n_rows, "position_ids")
         _index(seq_lens, torch.int32, n_seqs, "seq_lens")
         _index(cu_rows, torch.int32, n_seqs + 1, "cu_rows")
         self._launch(dev, self.lib.sq_rope_kv_write_paged, "sq_rope_kv_write_paged",
-                     (qkv.data_ptr(), qkv.stride(0) if n_rows > 1 else qkv.shape[1], q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                      _ptr(k_scales), _ptr(v_scales), cos.data_ptr(), sin.data_ptr(), cos.shape[0], position_ids.data_ptr(),
+                     (qkv.data_ptr(), stride[0] if n_rows > 1 else cols, q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                      _ptr(k_scales), _ptr(v_scales), cos.data_ptr(), sin.data_ptr(), table[0], position_ids.data_ptr(),
                       page_table.data_ptr(), width, n_pages, page_size, seq_lens.data_ptr(), cu_rows.data_ptr(), n_seqs, n_rows, n_heads,
                       h_kv, d, _DTYPE_CODES[dt]))
 
@@ -478,12 +480,13 @@ class HipOps:
         max_count: no sequence asks for more rows (default: M); rows beyond it are not read."""
         dev, dt = k_out.device, k_out.dtype
         _on_device(dev, k_pages, v_pages, v_out, page_table, starts, counts, k_scales, v_scales)
-        if dt not in (torch.float16, torch.bfloat16) or v_out.dtype != dt:
+        if (dt is not torch.float16 and dt is not torch.bfloat16) or v_out.dtype is not dt:
             raise TypeError(f"k_out / v_out: expected torch.float16 or torch.bfloat16 twice, got {dt}, {v_out.dtype}")
         n_pages, h_kv, page_size, d, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
-        if k_out.dim() != 4 or (k_out.shape[0], k_out.shape[1], k_out.shape[3]) != (n_seqs, h_kv, d) or v_out.shape != k_out.shape:
-            raise ValueError(f"k_out / v_out: expected [{n_seqs}, {h_kv}, M, {d}] twice, got {tuple(k_out.shape)}, {tuple(v_out.shape)}")
-        m = k_out.shape[2]
+        shape = k_out.shape
+        if len(shape) != 4 or shape[0] != n_seqs or shape[1] != h_kv or shape[3] != d or v_out.shape != shape:
+            raise ValueError(f"k_out / v_out: expected [{n_seqs}, {h_kv}, M, {d}] twice, got {tuple(shape)}, {tuple(v_out.shape)}")
+        m = shape[2]
         s = k_out.stride()
         if v_out.stride() != s or s[3] != 1 or (m > 1 and s[2] != d) or (h_kv > 1 and s[1] < m * d) or (n_seqs > 1 and s[0] < m * d):
             raise ValueError(f"k_out / v_out: expected contiguous rows and the same strides, got {s}, {v_out.stride()}")
@@ -507,14 +510,16 @@ class HipOps:
         may be.  The default max_len costs workgroups that find nothing to do."""
         dev, dt = q.device, q.dtype
         _on_device(dev, k_pages, v_pages, out, page_table, seq_lens, cu_rows, k_scales, v_scales)
-        if dt not in (torch.float16, torch.bfloat16) or out.dtype != dt:
+        if (dt is not torch.float16 and dt is not torch.bfloat16) or out.dtype is not dt:
             raise TypeError(f"q / out: expected torch.float16 or torch.bfloat16 twice, got {dt}, {out.dtype}")
         n_pages, h_kv, page_size, d, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
-        if q.dim() != 3 or q.shape[2] != d or q.shape[0] % h_kv or q.stride(2) != 1:
-            raise ValueError(f"q: expected [H, n_rows, {d}] with unit inner stride and a multiple of {h_kv} heads, got {tuple(q.shape)}")
-        n_heads, n_rows = q.shape[0], q.shape[1]
-        if out.shape != (n_rows, n_heads * d) or out.stride(1) != 1 or (n_rows > 1 and out.stride(0) < n_heads * d):
-            raise ValueError(f"out: expected {(n_rows, n_heads * d)} with unit inner stride, got {tuple(out.shape)}")
+        shape, stride = q.shape, q.stride()
+        if len(shape) != 3 or shape[2] != d or not h_kv or shape[0] % h_kv or stride[2] != 1:
+            raise ValueError(f"q: expected [H, n_rows, {d}] with unit inner stride and a multiple of {h_kv} heads, got {tuple(shape)}")
+        n_heads, n_rows = shape[0], shape[1]
+        cols, out_stride = n_heads * d, out.stride()
+        if out.shape != (n_rows, cols) or out_stride[1] != 1 or (n_rows > 1 and out_stride[0] < cols):
+            raise ValueError(f"out: expected {(n_rows, cols)} with unit inner stride, got {tuple(out.shape)}")
         _index(seq_lens, torch.int32, n_seqs, "seq_lens")
         _index(cu_rows, torch.int32, n_seqs + 1, "cu_rows")
         max_rows = n_rows if max_rows is None else min(int(max_rows), n_rows)
@@ -527,8 +532,8 @@ class HipOps:
         # one buffer a call, from the stream-ordered allocator: two streams or two captured graphs never share it
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         self._launch(dev, self.lib.sq_paged_attention, "sq_paged_attention",
-                     (q.data_ptr(), q.stride(0) if n_heads > 1 else 0, q.stride(1) if n_rows > 1 else 0, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
-                      out.data_ptr(), out.stride(0) if n_rows > 1 else n_heads * d, page_table.data_ptr(), width, n_pages, page_size,
+                     (q.data_ptr(), stride[0] if n_heads > 1 else 0, stride[1] if n_rows > 1 else 0, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+                      out.data_ptr(), out_stride[0] if n_rows > 1 else cols, page_table.data_ptr(), width, n_pages, page_size,
                       seq_lens.data_ptr(), cu_rows.data_ptr(), n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d, float(scale),
                       _DTYPE_CODES[dt], _ptr(ws), need))
         return out
@@ -543,16 +548,16 @@ class HipOps:
         dev, dt = target_logits.device, target_logits.dtype
         temps = temperature if isinstance(temperature, torch.Tensor) else None
         _on_device(dev, draft_logits, draft_tokens, cu_drafts, u_accept, u_next, temps, n_accepted, next_tokens)
-        if dt not in _DTYPE_CODES or draft_logits.dtype != dt:
+        if dt not in _DTYPE_CODES or draft_logits.dtype is not dt:
             raise TypeError(f"target_logits / draft_logits: expected fp16, bf16 or fp32 twice, got {dt}, {draft_logits.dtype}")
         n_seqs, n_drafts = n_accepted.shape[0], draft_tokens.shape[0]
-        if target_logits.dim() != 2 or draft_logits.dim() != 2 or target_logits.shape[1] != draft_logits.shape[1]:
-            raise ValueError(f"target_logits / draft_logits: expected two dimensions and one vocabulary, got {tuple(target_logits.shape)}, "
-                             f"{tuple(draft_logits.shape)}")
-        vocab = target_logits.shape[1]
-        for t, rows, name in ((target_logits, n_drafts + n_seqs, "target_logits"), (draft_logits, n_drafts, "draft_logits")):
-            if t.shape[0] < rows or (rows and t.stride(1) != 1) or (rows > 1 and t.stride(0) < vocab):
-                raise ValueError(f"{name}: expected {rows} rows with unit inner stride, got {tuple(t.shape)}")
+        t_shape, d_shape, t_stride, d_stride = target_logits.shape, draft_logits.shape, target_logits.stride(), draft_logits.stride()
+        if len(t_shape) != 2 or len(d_shape) != 2 or t_shape[1] != d_shape[1]:
+            raise ValueError(f"target_logits / draft_logits: expected two dimensions and one vocabulary, got {tuple(t_shape)}, {tuple(d_shape)}")
+        vocab = t_shape[1]
+        for shape, stride, rows, name in ((t_shape, t_stride, n_drafts + n_seqs, "target_logits"), (d_shape, d_stride, n_drafts, "draft_logits")):
+            if shape[0] < rows or (rows and stride[1] != 1) or (rows > 1 and stride[0] < vocab):
+                raise ValueError(f"{name}: expected {rows} rows with unit inner stride, got {tuple(shape)}")
         _index(draft_tokens, torch.int64, n_drafts, "draft_tokens")
         _index(cu_drafts, torch.int32, n_seqs + 1, "cu_drafts")
         _index(u_accept, torch.float32, n_drafts, "u_accept")
@@ -566,8 +571,8 @@ class HipOps:
         need = self._verify_workspace(n_seqs, n_drafts, vocab)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         self._launch(dev, self.lib.sq_verify_drafts, "sq_verify_drafts",
-                     (target_logits.data_ptr(), max(target_logits.stride(0), vocab), _ptr(draft_logits) or None,
-                      max(draft_logits.stride(0), vocab), _ptr(draft_tokens) or None, cu_drafts.data_ptr(), n_seqs, n_drafts, vocab,
+                     (target_logits.data_ptr(), max(t_stride[0], vocab), _ptr(draft_logits) or None,
+                      max(d_stride[0], vocab), _ptr(draft_tokens) or None, cu_drafts.data_ptr(), n_seqs, n_drafts, vocab,
                       _ptr(u_accept) or None, u_next.data_ptr(), _ptr(temps), 0.0 if temps is not None else float(temperature),
                       n_accepted.data_ptr(), next_tokens.data_ptr(), _DTYPE_CODES[dt], ws.data_ptr(), need))
         return n_accepted, next_tokens
