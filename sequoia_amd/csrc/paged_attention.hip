@@ -125,18 +125,27 @@ __device__ __forceinline__ size_t stored_row(const PagedAttnParams& P, int page,
 // The keys of all units, in order, are shared out evenly over the workgroups that fit the card, in steps of 128: a workgroup takes
 // the end of one unit, whole ones, and the beginning of another, and leaves the sums of the first and the last for the join;
 // whatever the lengths, all of them end together.  The next chunk's rows are asked for as soon as this one's have left their
-// registers, the next unit's while this one's waves join.  (Two workgroups a CU: three read 10 % slower.)
+// registers, the next unit's first ones too: it is looked up when this one begins.  (Two workgroups a CU: three read 10 % slower.)
+// Sequences of few hundred keys pay for the waves' joins: 2048 of 50-300 keys, 64 / 8 heads, fp16, 437 us (3.4 TB/s), 512 of 100-900
+// 213 us (4.8), 200 of 1000-3000 285 us (6.0).
 #define PAD_NW 4
 #define PAD_BK 32
 #define PAD_STEP (PAD_NW * PAD_BK)
 
 // the packed rows of sequence b, their first row, stored rows and key end; offsets that name no rows: none
 struct Rows { int first, rows, past, end; };
-__device__ __forceinline__ Rows rows_of_seq(const PagedAttnParams& P, int b) {
+// UNIFORM: by the scalar unit, so that no vector load in flight is waited for
+template <bool UNIFORM = false> __device__ __forceinline__ Rows rows_of_seq(const PagedAttnParams& P, int b) {
+    typedef const __attribute__((address_space(4))) int32_t* scalar;
     Rows R;
-    R.first = P.cu_rows[b];
-    const int n = P.cu_rows[b + 1] - R.first;
-    R.past = P.seq_lens[b];
+    int upto;
+    if constexpr (UNIFORM) {
+        const scalar cu = (scalar)(uintptr_t)(P.cu_rows + b), lens = (scalar)(uintptr_t)(P.seq_lens + b);
+        R.first = cu[0]; upto = cu[1]; R.past = lens[0];
+    } else {
+        R.first = P.cu_rows[b]; upto = P.cu_rows[b + 1]; R.past = P.seq_lens[b];
+    }
+    const int n = upto - R.first;
     R.rows = R.first >= 0 && n > 0 && n <= P.n_rows - R.first ? n * P.group : 0;
     R.end = R.rows ? attn_tile_end(P, R.past, R.rows, 0, P.tile_rows) : 0;
     return R;
@@ -199,23 +208,18 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
     } else {
         seq = blockIdx.x / P.h_kv;
     }
-    Rows R;
-    int steps, upto, k0, k1, lim0;
-    auto at_seq = [&]() {
-        const Rows r = rows_of_seq(P, seq);
-        R.first = __builtin_amdgcn_readfirstlane(r.first);
-        R.rows = __builtin_amdgcn_readfirstlane(r.rows < ROWS ? r.rows : ROWS);
-        R.past = __builtin_amdgcn_readfirstlane(r.past);
-        R.end = __builtin_amdgcn_readfirstlane(r.end);
-        steps = steps_of(R.end);
-        lim0 = R.past;                              // keys up to here are seen by every row
+    auto at_seq = [&](int b, Rows& r) {             // -> the steps of one of its units
+        r = rows_of_seq<true>(P, b);
+        r.rows = r.rows < ROWS ? r.rows : ROWS;
+        return steps_of(r.end);
     };
+    Rows R;
+    int steps = at_seq(seq, R), upto, k0, k1;
     auto at_unit = [&]() {
         upto = left < steps - from ? from + left : steps;
         k0 = from * PAD_STEP;
         k1 = R.end < upto * PAD_STEP ? R.end : upto * PAD_STEP;
     };
-    at_seq();
     if (P.n_groups) {
         kvh = from / steps;
         from -= kvh * steps;
@@ -230,15 +234,16 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
     uint32_t ksr[PASSES], vsr[PASSES];
     size_t row[2];                                  // scalar: first rows of the chunk's halves
     int ea = 0, eb = 0;                             // entries of the pages that hold the halves of the next chunk
+    int na = 0, nb = 0;                             // of the next unit's first one
     v8 qf[MT][DSTEPS];
     int lim[MT];                                    // last key this lane's query row sees, here
-    auto pages = [&](int key0, int& a, int& b) {
-        a = page_entry(P.map, seq, key0 >> P.map.shift);
-        b = page_entry(P.map, seq, (key0 + 16) >> P.map.shift);
+    auto pages = [&](int of_seq, int key0, int& a, int& b) {
+        a = page_entry(P.map, of_seq, key0 >> P.map.shift);
+        b = page_entry(P.map, of_seq, (key0 + 16) >> P.map.shift);
     };
-    auto take = [&](int key0, int a, int b) {
-        row[0] = stored_row(P, check_page(P.map, a), kvh, key0);
-        row[1] = stored_row(P, check_page(P.map, b), kvh, key0 + 16);
+    auto take = [&](int of_kvh, int key0, int a, int b) {
+        row[0] = stored_row(P, check_page(P.map, a), of_kvh, key0);
+        row[1] = stored_row(P, check_page(P.map, b), of_kvh, key0 + 16);
     };
     auto load = [&]() {
 #pragma unroll
@@ -264,9 +269,9 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
     };
     {
         int fa, fb;
-        pages(k0 + wave * PAD_BK, fa, fb);
-        pages(k0 + wave * PAD_BK + PAD_STEP, ea, eb);
-        take(k0 + wave * PAD_BK, fa, fb);           // (a wave without a chunk here loads one all the same, in bounds)
+        pages(seq, k0 + wave * PAD_BK, fa, fb);
+        pages(seq, k0 + wave * PAD_BK + PAD_STEP, ea, eb);
+        take(kvh, k0 + wave * PAD_BK, fa, fb);      // (a wave without a chunk here loads one all the same, in bounds)
         load();
         load_q();
     }
@@ -276,6 +281,17 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int s = 0; s < DSTEPS; ++s) arrived(qf[mt][s]);
+        // the next unit, looked up while this one's first rows are on their way: its own first rows follow this one's last
+        int nseq = seq, nkvh = kvh + 1, nsteps = steps;
+        Rows nR = R;
+        bool next = P.n_groups && left > upto - from;
+        if (next && nkvh == P.h_kv) {
+            nkvh = 0;
+            do ++nseq; while (nseq < P.n_seqs && (nsteps = at_seq(nseq, nR)) == 0);
+            next = nseq < P.n_seqs;
+        }
+        if (next) pages(nseq, wave * PAD_BK, na, nb);
+        const int lim0 = R.past;                    // keys up to here are seen by every row
         float m_run[MT], l_run[MT];
         floatx4 o_acc[MT][NT];
 #pragma unroll
@@ -315,11 +331,11 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
                         for (int j = 0; j < RPP; ++j) hidden |= (uint32_t)(((lanes >> (j * LPR)) & ((1ull << LPR) - 1)) != 0) << (i * RPP + j);
                 }
             }
-            if (more) {                             // the entries of the chunk after the next come first: loads end in order
-                const int fa = ea, fb = eb;
-                pages(key0 + 2 * PAD_STEP, ea, eb);
-                take(key0 + PAD_STEP, fa, fb);
-                load();
+            {                                       // the entries of the chunk after the next come first: loads end in order
+                const int key = more ? key0 + PAD_STEP : wave * PAD_BK;
+                take(more ? kvh : nkvh, key, more ? ea : na, more ? eb : nb);
+                pages(more || !next ? seq : nseq, key + PAD_STEP, ea, eb);
+                if (more || next) load();
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -397,28 +413,24 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
             __builtin_amdgcn_wave_barrier();
         }
 
-        // ---- join the waves, with the next unit's first loads on their way ----
+        if (next && k0 + wave * PAD_BK >= k1) {     // a wave without a chunk of this unit
+            take(nkvh, wave * PAD_BK, na, nb);
+            pages(nseq, wave * PAD_BK + PAD_STEP, ea, eb);
+            load();
+        }
+
+        // ---- join the waves, with the next unit's first rows on their way ----
         const bool whole = from == 0 && upto == steps;
         const int done_rows = R.rows, done_first = R.first, done_head = kvh * P.group;
         if (P.n_groups && from == 0 && tid == 0) {  // where the join finds the unit's parts
             int2* const u = P.units + seq * P.h_kv + kvh;
             *u = int2{(int)(2 * blockIdx.x + (first_unit ? 0 : 1)), whole ? 1 : 1 + (steps - upto + per - 1) / per};
         }
-        left -= upto - from;
-        bool next = P.n_groups && left > 0;
         if (next) {
+            left -= upto - from;
             from = 0;
-            if (++kvh == P.h_kv) {
-                kvh = 0;
-                do ++seq; while (seq < P.n_seqs && (at_seq(), steps == 0));
-                next = seq < P.n_seqs;
-            }
-        }
-        int fa = 0, fb = 0;
-        if (next) {
+            seq = nseq; kvh = nkvh; steps = nsteps; R = nR;
             at_unit();
-            pages(k0 + wave * PAD_BK, fa, fb);
-            pages(k0 + wave * PAD_BK + PAD_STEP, ea, eb);
         }
         __syncthreads();                            // everyone is done with the staging area
         float* lds_o = (float*)lds;
@@ -430,11 +442,7 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
             for (int nt = 0; nt < NT; ++nt) *(floatx4*)(lds_o + (wave * ROWS + 16 * mt + qc) * OSTR + 16 * nt + 4 * g) = o_acc[mt][nt];
         }
         __syncthreads();
-        if (next) {
-            take(k0 + wave * PAD_BK, fa, fb);
-            load();
-            load_q();
-        }
+        if (next) load_q();
         for (int e = tid; e < ROWS * (D / 4); e += PAD_NW * 64) {
             const int r = e / (D / 4), col = 4 * (e % (D / 4));
             if (r >= done_rows) break;              // rows ascend with e
