@@ -1,10 +1,12 @@
-"""Build libsequoia_hip.so (gfx950) in-tree with hipcc.  `python -m sequoia_amd.build`."""
+"""Build libsequoia_hip.so (gfx950) in-tree with hipcc, and the paged operators' binding with the host compiler.  `python -m sequoia_amd.build`."""
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -41,6 +43,23 @@ def _stale(target: str, deps: list[str]) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+# the paged operators' binding to torch tensors: host code, against the headers of the torch that is installed
+BINDING = os.path.join(LIBDIR, "_paged.so")
+BINDING_SOURCE = os.path.join(CSRC, "paged_binding.cpp")
+
+
+def build_binding(force: bool = False, verbose: bool = True) -> str:
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    if force or _stale(BINDING, [BINDING_SOURCE, os.path.join(os.path.dirname(PKG), "include", "sequoia_hip.h"), os.path.join(torch, "version.py")]):
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-isystem", os.path.join(torch, "include"),
+               "-isystem", os.path.join(torch, "include", "torch", "csrc", "api", "include"), "-isystem", sysconfig.get_paths()["include"],
+               BINDING_SOURCE, "-o", BINDING, "-L" + os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = True) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     srcs = [os.path.join(CSRC, s) for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
@@ -60,6 +79,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+    build_binding(force, verbose)
     return LIB
 
 

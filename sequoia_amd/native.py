@@ -149,6 +149,35 @@ def load() -> C.CDLL:
     return lib
 
 
+PAGED_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_paged.so")
+_PAGED_ENTRIES = ("sq_rope_kv_write_paged", "sq_kv_read_paged", "sq_paged_attention_workspace_bytes", "sq_paged_attention",
+                  "sq_verify_drafts_workspace_bytes", "sq_verify_drafts")
+_paged_callbacks = []
+
+
+def load_paged(lib):
+    """The binding of the paged operators (csrc/paged_binding.cpp) on `lib`'s entries."""
+    if not os.path.exists(PAGED_PATH):
+        raise SequoiaNativeError(f"{PAGED_PATH} not found: build it with `python -m sequoia_amd.build`")
+    import importlib.machinery
+    import importlib.util
+    import torch
+    loader = importlib.machinery.ExtensionFileLoader("_paged", PAGED_PATH)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_paged", loader))
+    loader.exec_module(module)
+
+    def address(name):
+        fn = getattr(lib, name)
+        if isinstance(lib, _TracedLib):                     # the binding calls back into the traced call
+            res, args = PROTOTYPES[name]
+            fn = C.CFUNCTYPE(res, *args)(fn)
+            _paged_callbacks.append(fn)
+        return C.cast(fn, C.c_void_p).value
+
+    module.bind(*(address(name) for name in _PAGED_ENTRIES), torch._C._cuda_getCurrentRawStream, check, SequoiaNativeError)
+    return module
+
+
 class _TracedLib:
     """Debug aid (SEQUOIA_TRACE_CALLS=1): every C-ABI call is announced on stderr BEFORE it runs and followed by a device
     synchronisation, so that a GPU memory fault (which aborts the process asynchronously) names the entry point it happened

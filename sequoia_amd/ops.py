@@ -34,61 +34,16 @@ def _need(t: torch.Tensor, dtype, name: str, contiguous: bool = True):
     return t
 
 
-_DTYPE_CODES = {torch.float16: native.SQ_DTYPE_F16, torch.bfloat16: native.SQ_DTYPE_BF16, torch.float32: native.SQ_DTYPE_F32}
-
-
-def _on_device(dev, *tensors):
-    """Every tensor (None is allowed) on the device `dev` of the call: the launch goes to that device's current stream."""
-    if dev.type != "cuda":
-        raise native.SequoiaNativeError(f"the tensors live on {dev}: the paged path only runs on a HIP device (no CPU fallback)")
-    index = dev.index
-    for t in tensors:
-        if t is not None and t.get_device() != index:
-            raise ValueError(f"the call's tensors live on different devices: {[str(x.device) for x in tensors if x is not None]} beside {dev}")
-
-
-def _index(t, dtype, n, name):
-    if t.dtype is not dtype:
-        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    shape = t.shape
-    if len(shape) != 1 or shape[0] < n or not t.is_contiguous():
-        raise ValueError(f"{name}: expected {n} contiguous entries, got {tuple(shape)}")
-
-
-def _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dtype):
-    """Checks the pages of one layer; -> (n_pages, H_kv, page_size, D, sequences, table width)."""
-    shape = k_pages.shape
-    if len(shape) != 4 or v_pages.shape != shape:
-        raise ValueError(f"k_pages / v_pages: expected [n_pages, H_kv, page_size, D] twice, got {tuple(shape)}, {tuple(v_pages.shape)}")
-    want = dtype if k_scales is None else torch.float8_e4m3fn
-    if k_pages.dtype is not want or v_pages.dtype is not want:
-        raise TypeError(f"k_pages / v_pages: expected {want}, got {k_pages.dtype}, {v_pages.dtype}")
-    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
-        raise ValueError("k_pages / v_pages: must be contiguous")
-    if (k_scales is None) != (v_scales is None):
-        raise ValueError("k_scales / v_scales: both or none")
-    if k_scales is not None:
-        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
-            if t.dtype is not torch.uint8:
-                raise TypeError(f"{name}: expected torch.uint8, got {t.dtype}")
-            if t.shape != shape[:3] or not t.is_contiguous():
-                raise ValueError(f"{name}: expected {tuple(shape[:3])} contiguous, got {tuple(t.shape)}")
-    if page_table.dtype is not torch.int32:
-        raise TypeError(f"page_table: expected torch.int32, got {page_table.dtype}")
-    table = page_table.shape
-    if len(table) != 2 or not page_table.is_contiguous():
-        raise ValueError(f"page_table: expected [sequences, pages] contiguous, got {tuple(table)}")
-    return (*shape, *table)
-
-
 class HipOps:
     name = "hip"
 
     def __init__(self):
         self.lib = native.load()
-        # sizes of sizes: the layers of a step ask for the same
-        self._attention_workspace = functools.lru_cache(256)(self.lib.sq_paged_attention_workspace_bytes)
-        self._verify_workspace = functools.lru_cache(256)(self.lib.sq_verify_drafts_workspace_bytes)
+
+    @functools.cached_property
+    def _paged(self):
+        """csrc/paged_binding.cpp: checks, workspace and call of the paged operators, on the current stream of the tensors' device."""
+        return native.load_paged(self.lib)
 
     @staticmethod
     def _stream():
@@ -429,77 +384,19 @@ class HipOps:
         return result
 
     # ---- batched speculative decoding over a paged KV cache -------------------------------------
-    @staticmethod
-    def _launch(dev, fn, what, args):
-        """fn(*args, stream) on `dev`'s current stream, with `dev` current for the launch."""
-        # the raw handle: torch.cuda.current_stream() builds a Stream object, 2.7 us of a small call's 13
-        index = dev.index
-        if index == torch._C._cuda_getDevice():
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-        else:
-            with torch.cuda.device(dev):
-                rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-        if rc:
-            check(rc, what)
-
     def rope_kv_write_paged(self, qkv, q_out, k_pages, v_pages, cos, sin, position_ids, page_table, seq_lens, cu_rows, n_heads, h_kv,
                             d, k_scales=None, v_scales=None):
         """RoPE of the packed rows qkv [n_rows, (H + 2 H_kv) D] of a ragged batch into q_out [H, n_rows, D], and the write of K and
         V behind each sequence's stored rows: row cu_rows[b] + i goes to row seq_lens[b] + i of sequence b.  Pages
         [n_pages, H_kv, page_size, D] in qkv's type, or float8_e4m3fn with k_scales / v_scales (uint8, [n_pages, H_kv, page_size]).
         Rows behind cu_rows[-1] are left alone."""
-        dev, dt = qkv.device, qkv.dtype
-        _on_device(dev, q_out, k_pages, v_pages, cos, sin, position_ids, page_table, seq_lens, cu_rows, k_scales, v_scales)
-        if dt is not torch.float16 and dt is not torch.bfloat16:
-            raise TypeError(f"qkv: expected torch.float16 or torch.bfloat16, got {dt}")
-        if q_out.dtype is not dt or cos.dtype is not dt or sin.dtype is not dt:
-            raise TypeError(f"q_out / cos / sin: expected {dt} three times, got {q_out.dtype}, {cos.dtype}, {sin.dtype}")
-        n_pages, hk, page_size, dim, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
-        shape, stride, cols = qkv.shape, qkv.stride(), (n_heads + 2 * h_kv) * d
-        if len(shape) != 2 or stride[1] != 1 or shape[1] != cols or hk != h_kv or dim != d:
-            raise ValueError(f"qkv: expected [n_rows, {cols}] with unit inner stride over pages of {h_kv} heads of {d}, "
-                             f"got {tuple(shape)} over {hk} heads of {dim}")
-        n_rows = shape[0]
-        if q_out.shape != (n_heads, n_rows, d) or not q_out.is_contiguous():
-            raise ValueError(f"q_out: expected {(n_heads, n_rows, d)} contiguous, got {tuple(q_out.shape)}")
-        table = cos.shape
-        if len(table) != 2 or table[1] != d or table != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
-            raise ValueError(f"cos / sin: expected [positions, {d}] contiguous twice, got {tuple(table)}, {tuple(sin.shape)}")
-        _index(position_ids, torch.int64, n_rows, "position_ids")
-        _index(seq_lens, torch.int32, n_seqs, "seq_lens")
-        _index(cu_rows, torch.int32, n_seqs + 1, "cu_rows")
-        self._launch(dev, self.lib.sq_rope_kv_write_paged, "sq_rope_kv_write_paged",
-                     (qkv.data_ptr(), stride[0] if n_rows > 1 else cols, q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                      _ptr(k_scales), _ptr(v_scales), cos.data_ptr(), sin.data_ptr(), table[0], position_ids.data_ptr(),
-                      page_table.data_ptr(), width, n_pages, page_size, seq_lens.data_ptr(), cu_rows.data_ptr(), n_seqs, n_rows, n_heads,
-                      h_kv, d, _DTYPE_CODES[dt]))
+        self._paged.write(qkv, q_out, k_pages, v_pages, cos, sin, position_ids, page_table, seq_lens, cu_rows, n_heads, h_kv, d, k_scales, v_scales)
 
     def kv_read_paged(self, k_pages, v_pages, k_out, v_out, page_table, starts, counts, max_count=None, k_scales=None, v_scales=None):
         """Stored rows [starts[b], starts[b] + counts[b]) of every sequence into rows [0, counts[b]) of k_out / v_out
         [sequences, H_kv, M, D] (fp16 or bf16, rows contiguous: layer slabs of static caches fit).  Other rows stay as they are.
         max_count: no sequence asks for more rows (default: M); rows beyond it are not read."""
-        dev, dt = k_out.device, k_out.dtype
-        _on_device(dev, k_pages, v_pages, v_out, page_table, starts, counts, k_scales, v_scales)
-        if (dt is not torch.float16 and dt is not torch.bfloat16) or v_out.dtype is not dt:
-            raise TypeError(f"k_out / v_out: expected torch.float16 or torch.bfloat16 twice, got {dt}, {v_out.dtype}")
-        n_pages, h_kv, page_size, d, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
-        shape = k_out.shape
-        if len(shape) != 4 or shape[0] != n_seqs or shape[1] != h_kv or shape[3] != d or v_out.shape != shape:
-            raise ValueError(f"k_out / v_out: expected [{n_seqs}, {h_kv}, M, {d}] twice, got {tuple(shape)}, {tuple(v_out.shape)}")
-        m = shape[2]
-        s = k_out.stride()
-        if v_out.stride() != s or s[3] != 1 or (m > 1 and s[2] != d) or (h_kv > 1 and s[1] < m * d) or (n_seqs > 1 and s[0] < m * d):
-            raise ValueError(f"k_out / v_out: expected contiguous rows and the same strides, got {s}, {v_out.stride()}")
-        _index(starts, torch.int32, n_seqs, "starts")
-        _index(counts, torch.int32, n_seqs, "counts")
-        if max_count is None:
-            max_count = m
-        if not 0 <= max_count <= m:
-            raise ValueError(f"max_count: {max_count} is not between 0 and {m}")
-        self._launch(dev, self.lib.sq_kv_read_paged, "sq_kv_read_paged",
-                     (k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), k_out.data_ptr(), v_out.data_ptr(),
-                      s[0] if n_seqs > 1 else h_kv * m * d, s[1] if h_kv > 1 else m * d, m, page_table.data_ptr(), width, n_pages, page_size,
-                      starts.data_ptr(), counts.data_ptr(), n_seqs, int(max_count), h_kv, d, _DTYPE_CODES[dt]))
+        self._paged.read(k_pages, v_pages, k_out, v_out, page_table, starts, counts, max_count, k_scales, v_scales)
         return k_out, v_out
 
     def paged_attention(self, q, k_pages, v_pages, out, page_table, seq_lens, cu_rows, scale, max_rows=None, max_len=None, k_scales=None,
@@ -508,34 +405,7 @@ class HipOps:
         sees keys [0, seq_lens[b] + i] of sequence b; out [n_rows, H D].  max_rows / max_len: no sequence brings more rows / ends
         behind more keys (defaults and caps: n_rows, the table's whole width); they size the launch; keys beyond them are left out, rows
         may be.  The default max_len costs workgroups that find nothing to do."""
-        dev, dt = q.device, q.dtype
-        _on_device(dev, k_pages, v_pages, out, page_table, seq_lens, cu_rows, k_scales, v_scales)
-        if (dt is not torch.float16 and dt is not torch.bfloat16) or out.dtype is not dt:
-            raise TypeError(f"q / out: expected torch.float16 or torch.bfloat16 twice, got {dt}, {out.dtype}")
-        n_pages, h_kv, page_size, d, n_seqs, width = _page_pool(k_pages, v_pages, k_scales, v_scales, page_table, dt)
-        shape, stride = q.shape, q.stride()
-        if len(shape) != 3 or shape[2] != d or not h_kv or shape[0] % h_kv or stride[2] != 1:
-            raise ValueError(f"q: expected [H, n_rows, {d}] with unit inner stride and a multiple of {h_kv} heads, got {tuple(shape)}")
-        n_heads, n_rows = shape[0], shape[1]
-        cols, out_stride = n_heads * d, out.stride()
-        if out.shape != (n_rows, cols) or out_stride[1] != 1 or (n_rows > 1 and out_stride[0] < cols):
-            raise ValueError(f"out: expected {(n_rows, cols)} with unit inner stride, got {tuple(out.shape)}")
-        _index(seq_lens, torch.int32, n_seqs, "seq_lens")
-        _index(cu_rows, torch.int32, n_seqs + 1, "cu_rows")
-        max_rows = n_rows if max_rows is None else min(int(max_rows), n_rows)
-        max_len = width * page_size if max_len is None else min(int(max_len), width * page_size)
-        if max_rows < 0 or max_len < 0:
-            raise ValueError(f"max_rows {max_rows} / max_len {max_len}: expected bounds >= 0")
-        if not 0.0 < scale < float("inf"):
-            raise ValueError(f"scale: expected a positive number, got {scale}")
-        need = self._attention_workspace(n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d)
-        # one buffer a call, from the stream-ordered allocator: two streams or two captured graphs never share it
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        self._launch(dev, self.lib.sq_paged_attention, "sq_paged_attention",
-                     (q.data_ptr(), stride[0] if n_heads > 1 else 0, stride[1] if n_rows > 1 else 0, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
-                      out.data_ptr(), out_stride[0] if n_rows > 1 else cols, page_table.data_ptr(), width, n_pages, page_size,
-                      seq_lens.data_ptr(), cu_rows.data_ptr(), n_seqs, n_rows, max_rows, max_len, n_heads, h_kv, d, float(scale),
-                      _DTYPE_CODES[dt], _ptr(ws), need))
+        self._paged.attention(q, k_pages, v_pages, out, page_table, seq_lens, cu_rows, scale, max_rows, max_len, k_scales, v_scales)
         return out
 
     def verify_drafts(self, target_logits, draft_logits, draft_tokens, cu_drafts, u_accept, u_next, temperature, n_accepted, next_tokens):
@@ -545,36 +415,7 @@ class HipOps:
         u_accept q(token) < p(token); then the next token is drawn with u_next[b] from max(p - q, 0), or from p behind the last one.
         temperature: a number or a float32 tensor [sequences]; 0 is greedy.  n_accepted int32 / next_tokens int64 [sequences]
         (-1: the deciding row is no distribution)."""
-        dev, dt = target_logits.device, target_logits.dtype
-        temps = temperature if isinstance(temperature, torch.Tensor) else None
-        _on_device(dev, draft_logits, draft_tokens, cu_drafts, u_accept, u_next, temps, n_accepted, next_tokens)
-        if dt not in _DTYPE_CODES or draft_logits.dtype is not dt:
-            raise TypeError(f"target_logits / draft_logits: expected fp16, bf16 or fp32 twice, got {dt}, {draft_logits.dtype}")
-        n_seqs, n_drafts = n_accepted.shape[0], draft_tokens.shape[0]
-        t_shape, d_shape, t_stride, d_stride = target_logits.shape, draft_logits.shape, target_logits.stride(), draft_logits.stride()
-        if len(t_shape) != 2 or len(d_shape) != 2 or t_shape[1] != d_shape[1]:
-            raise ValueError(f"target_logits / draft_logits: expected two dimensions and one vocabulary, got {tuple(t_shape)}, {tuple(d_shape)}")
-        vocab = t_shape[1]
-        for shape, stride, rows, name in ((t_shape, t_stride, n_drafts + n_seqs, "target_logits"), (d_shape, d_stride, n_drafts, "draft_logits")):
-            if shape[0] < rows or (rows and stride[1] != 1) or (rows > 1 and stride[0] < vocab):
-                raise ValueError(f"{name}: expected {rows} rows with unit inner stride, got {tuple(shape)}")
-        _index(draft_tokens, torch.int64, n_drafts, "draft_tokens")
-        _index(cu_drafts, torch.int32, n_seqs + 1, "cu_drafts")
-        _index(u_accept, torch.float32, n_drafts, "u_accept")
-        _index(u_next, torch.float32, n_seqs, "u_next")
-        _index(n_accepted, torch.int32, n_seqs, "n_accepted")
-        _index(next_tokens, torch.int64, n_seqs, "next_tokens")
-        if temps is not None:
-            _index(temps, torch.float32, n_seqs, "temperature")
-        elif not 0.0 <= temperature < float("inf"):
-            raise ValueError(f"temperature: expected a number >= 0, got {temperature}")
-        need = self._verify_workspace(n_seqs, n_drafts, vocab)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        self._launch(dev, self.lib.sq_verify_drafts, "sq_verify_drafts",
-                     (target_logits.data_ptr(), max(t_stride[0], vocab), _ptr(draft_logits) or None,
-                      max(d_stride[0], vocab), _ptr(draft_tokens) or None, cu_drafts.data_ptr(), n_seqs, n_drafts, vocab,
-                      _ptr(u_accept) or None, u_next.data_ptr(), _ptr(temps), 0.0 if temps is not None else float(temperature),
-                      n_accepted.data_ptr(), next_tokens.data_ptr(), _DTYPE_CODES[dt], ws.data_ptr(), need))
+        self._paged.verify(target_logits, draft_logits, draft_tokens, cu_drafts, u_accept, u_next, temperature, n_accepted, next_tokens)
         return n_accepted, next_tokens
 
     # ---- row-wise glue ------------------------------------------------------------------------
