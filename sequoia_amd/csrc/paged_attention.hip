@@ -41,6 +41,21 @@ template <typename T> __device__ __forceinline__ floatx16 mfma32(typename vec_of
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+// c + a[0] + a[1] + .. of a fragment's eight weights.  What the second product uses is what the sum is taken of, so that a weight's
+// rounding is one of the whole row's scale where that weight is most of the row, and not of the result.
+template <typename T> __device__ __forceinline__ float add_weights(typename vec_of<T>::v8 a, float c) {
+    typedef typename vec_of<T>::v2 v2;
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const v2 two = {a[i], a[i + 1]}, one = {(T)1.f, (T)1.f};
+        float& to = i & 2 ? d : c;
+        if constexpr (__is_same(T, half_t)) to = __builtin_amdgcn_fdot2(two, one, to, false);
+        else to = __builtin_amdgcn_fdot2_f32_bf16(two, one, to, false);
+    }
+    return c + d;
+}
+
 // column (lane & 15) of the 4 x 16 block of 16-bit values whose row (lane & 15) >> 2, columns 4 (lane & 3).. this lane addresses
 __device__ __forceinline__ u32x2 read_transposed(const void* p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)p));
@@ -483,8 +498,9 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
 //                  while no maximum of the wave moves.
 // Two workgroups share a CU, so that one's exponentials run beside the other's products.
 // A row's maximum is replaced only when it grows by more than a factor of 2^8: weights then reach 256 instead of 1, with the same
-// relative rounding to the element type and the same fp32 sum; what is lost is that the largest weight is no longer exactly 1, one
-// more rounding of half a step.  16-bit rows go global -> LDS without registers; e4m3 rows through registers, which widen them.
+// relative rounding to the element type and the same fp32 sum; what is lost is that the largest weight is no longer exactly 1, and
+// the sum of the rounded weights makes up for most of it (error against 64 bits 0.0017; 0.0019 with the sum of the unrounded ones;
+// 0.0016 of it is the output's own rounding).  16-bit rows go global -> LDS without registers; e4m3 rows through registers, which widen them.
 // 4096 rows of 64 heads behind 4001 stored ones, 8 KV heads of 128, bf16: 771 us, 1.05 PFLOP/s of the products that the mask leaves
 // (a large library product here: 1.26).  Of a wave's 2000 or so cycles a tile, 1024 are products; the exponentials and the
 // maximum's pass run beside the other wave's products only in part (a priority for one of the two changes nothing; three workgroups
@@ -673,16 +689,13 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
         }
         const float m_use = m_run == -INFINITY ? 0.f : m_run;
         v8 pf[KS];
-        float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s_acc[b][i], P.scale_log2e, -m_use));
-                sum += p;
-                pf[2 * b + (i >> 3)][i & 7] = (T)p;
-            }
-        l_run += sum;
+            for (int i = 0; i < 16; ++i)
+                pf[2 * b + (i >> 3)][i & 7] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s_acc[b][i], P.scale_log2e, -m_use));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) l_run = add_weights<T>(pf[ks], l_run);
         // slot (h, j) of step ks is key 16 ks + 8 (j >> 2) + 4 h + (j & 3): the order the weights stand in
         auto v_frag = [&](int ks, int b) {
             const int r = 4 * h + ((lane & 15) >> 2), c = 4 * b + ((lane >> 3) & 2) + ((lane & 3) >> 1);      // order(16 ks + r) = order(r)

@@ -57,6 +57,8 @@ def attention(q, k, v, past, scale, dtype):
     The bound, element by element (u = half a step of the element type, e = 2^-24, w_j the softmax weights):
       the output's rounding                          u |o|
       the weights' rounding for the second product   u sum w_j |v_j|, and below the type's normal range TINY each
+      where the sum is taken of the rounded weights, sum w_j (1 + a_j) v_j / sum w_j (1 + a_j) with |a_j| <= u is off by
+      sum w_j a_j (v_j - o) / sum w_j (1 + a_j): u |o| more, and TINY |o| each
       a score's fp32 sum of D exact products and its scaling, an exponential of 2 units in the last place, the exponent's own
       subtraction: each weight off by a factor 1 + d, d = 2 (D + 4) e scale sum |q_i k_ij| + 4 e |s| + 4 e; numerator and denominator
       fp32 sums over n keys (in blocks, but at worst) 2 (n + 8) e sum w_j |v_j|"""
@@ -78,8 +80,9 @@ def attention(q, k, v, past, scale, dtype):
     wv = torch.matmul(w, va)
     u = EPS[dtype]
     keys = kk.shape[1]
-    bound = u * o.abs() * (1 + u) + (u + 2 * off + 2 * (keys + 8) * e) * wv * (1 + u) + TINY[dtype]
-    bound = bound + TINY[dtype] * torch.matmul((~hidden).double().expand_as(w), va) / total
+    bound = 2 * u * o.abs() * (1 + 2 * u) + (u + 2 * off + 2 * (keys + 8) * e) * wv * (1 + 2 * u) + TINY[dtype]
+    seen = (~hidden).double().expand_as(w)
+    bound = bound + TINY[dtype] * (torch.matmul(seen, va) + seen.sum(-1, keepdim=True) * o.abs()) / total
     return o.transpose(0, 1), bound.transpose(0, 1)
 
 
