@@ -496,7 +496,8 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
 //                  two half-waves, and the weights are the second product's B operand where they stand
 //   O^T += V^T P^T V^T by transposing LDS reads; a lane's outputs belong to the same row: rescaling is lane-local, and skipped
 //                  while no maximum of the wave moves.
-// Two workgroups share a CU, so that one's exponentials run beside the other's products.
+// Two workgroups share a CU, so that one's exponentials run beside the other's products.  SHARED: at most a tile of rows a unit, and the
+// units' keys are shared out as the rows kernel's are.
 // A row's maximum is replaced only when it grows by more than a factor of 2^8: weights then reach 256 instead of 1, with the same
 // relative rounding to the element type and the same fp32 sum; what is lost is that the largest weight is no longer exactly 1, and
 // the sum of the rounded weights makes up for most of it (error against 64 bits 0.0017; 0.0019 with the sum of the unrounded ones;
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
 // a CU do not fit the registers).
 #define PAT_NW 4
 #define PAT_BK 64
-template <typename T, int D, bool Q8>
+template <typename T, int D, bool Q8, bool SHARED>
 __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(PagedAttnParams P) {
     typedef typename vec_of<T>::v8 v8;
     typedef typename vec_of<T>::v4 v4;
@@ -516,64 +517,90 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     constexpr int QS = D / 16, NB = D / 32, KS = PAT_BK / 16, ROWS = 32 * PAT_NW;
     __shared__ __attribute__((aligned(256))) unsigned char lds[2 * BUF * 2];
     __shared__ int lds_hidden[2][PAT_BK];           // rows of a tile with values that were taken out
-    AttnItem I;
-    if (!attn_item(P, ROWS, I)) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, qc = lane & 31, h = lane >> 5;
-    const int k0 = I.split * P.split_len, k1 = I.end < k0 + P.split_len ? I.end : k0 + P.split_len;
 
-    const int wrow = I.row0 + 32 * wave;            // the wave's first row
-    int r = wrow + qc;
-    const bool live = r < I.rows;
-    r = live ? r : I.rows - 1;
-    const int token = r / P.group, head = I.kvh * P.group + r - token * P.group;
-    int lim = I.past + token;                       // last key this lane's row sees, here
-    lim = lim < k1 ? lim : k1 - 1;
+    // ---- what it works on; SHARED: a share of all units' keys, as in the rows kernel ----
+    AttnItem I;
+    int k0, k1, from = 0, left = 0, per = 0, steps = 0, upto = 0;
+    auto at_unit = [&]() {
+        upto = left < steps - from ? from + left : steps;
+        k0 = from * PAD_STEP;
+        k1 = I.end < upto * PAD_STEP ? I.end : upto * PAD_STEP;
+    };
+    if constexpr (SHARED) {
+        int place = 0;
+        I.seq = __builtin_amdgcn_readfirstlane(share(P, blockIdx.x, per, place));
+        if (I.seq >= P.n_seqs) return;
+        left = per = __builtin_amdgcn_readfirstlane(per);
+        from = __builtin_amdgcn_readfirstlane(place);
+        const Rows R = rows_of_seq<true>(P, I.seq);
+        I.first = R.first; I.past = R.past; I.end = R.end; I.row0 = 0;
+        I.rows = R.rows < P.tile_rows ? R.rows : P.tile_rows;
+        steps = steps_of(R.end);
+        I.kvh = from / steps;
+        from -= I.kvh * steps;
+        at_unit();
+    } else {
+        if (!attn_item(P, ROWS, I)) return;
+        k0 = I.split * P.split_len;
+        k1 = I.end < k0 + P.split_len ? I.end : k0 + P.split_len;
+    }
+
+    // ---- the wave's rows ----
+    int r, token, head, lim, lim_lo, lim_hi, lim0;  // lim: last key this lane's row sees, here; lim0: keys up to it are seen by every row of the workgroup
+    bool live;
     v8 qf[QS];
-    {
+    auto enter = [&]() {
+        const int wrow = I.row0 + 32 * wave;        // the wave's first row
+        r = wrow + qc;
+        live = r < I.rows;
+        r = live ? r : I.rows - 1;
+        token = r / P.group; head = I.kvh * P.group + r - token * P.group;
+        lim = I.past + token;
+        lim = lim < k1 ? lim : k1 - 1;
         const T* qr = (const T*)P.q + head * P.q_head_stride + (size_t)(I.first + token) * P.q_row_stride + 8 * h;
 #pragma unroll
         for (int s = 0; s < QS; ++s) qf[s] = *(const v8*)(qr + 16 * s);
-    }
-    const int lim_of_row0 = I.past + I.row0 / P.group;
-    int wlast = wrow + 31 < I.rows ? wrow + 31 : I.rows - 1;
-    int lim_lo = I.past + wrow / P.group, lim_hi = I.past + wlast / P.group;
-    lim_lo = wrow < I.rows ? (lim_lo < k1 ? lim_lo : k1 - 1) : -1;      // a wave without rows only helps to fetch
-    lim_hi = wrow < I.rows ? (lim_hi < k1 ? lim_hi : k1 - 1) : -1;
+        const int lim_of_row0 = I.past + I.row0 / P.group;
+        int wlast = wrow + 31 < I.rows ? wrow + 31 : I.rows - 1;
+        lim_lo = I.past + wrow / P.group; lim_hi = I.past + wlast / P.group;
+        lim_lo = wrow < I.rows ? (lim_lo < k1 ? lim_lo : k1 - 1) : -1;      // a wave without rows only helps to fetch
+        lim_hi = wrow < I.rows ? (lim_hi < k1 ? lim_hi : k1 - 1) : -1;
+        lim0 = lim_of_row0 < k1 ? lim_of_row0 : k1 - 1;
+    };
+    enter();
 
-    float m_run = -INFINITY, l_run = 0.f;
+    float m_run, l_run;
     floatx16 o_acc[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) o_acc[i] = floatx16{};
 
     // Rows lie in LDS one behind the other, their 16-byte chunks in an order that depends on the row: chunk c of row r is at
     // place c ^ order(r).  The reads of K (one chunk of 16 consecutive rows) and the transposing reads of V (four chunks of four
     // consecutive rows) then touch every bank once, and rows can be fetched by loads that write LDS themselves.
     auto k_order = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
     auto v_order = [](int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 2) << 1) | ((r >> 2) & 3); };
-    const int lim0 = lim_of_row0 < k1 ? lim_of_row0 : k1 - 1;           // keys up to here are seen by every row of the workgroup
     const int lrow = lane / LPR, lcol = lane % LPR;
     // A wave's rows of a pass lie in one 16-row block, so in one page: its entry is uniform, the rows one behind the other.  Pages of
     // a tile's length or more hold all passes' rows: one look-up a tile instead of one a pass (60 scalar instructions of a tile's
     // 600 or so).
     constexpr int RPW = 64 / LPR;
     const bool whole = P.map.shift >= 6;
-    int pg[PASSES];
-    auto pages = [&](int key0) {
-        pg[0] = page_entry(P.map, I.seq, (key0 + wave * RPW) >> P.map.shift);
+    int pg[PASSES], npg[PASSES];                    // entries of the next tile; of the next unit's first one
+    auto pages = [&](int seq, int key0) {
+        pg[0] = page_entry(P.map, seq, (key0 + wave * RPW) >> P.map.shift);
         if (!whole) {
 #pragma unroll
-            for (int i = 1; i < PASSES; ++i) pg[i] = page_entry(P.map, I.seq, (key0 + i * RPP + wave * RPW) >> P.map.shift);
+            for (int i = 1; i < PASSES; ++i) pg[i] = page_entry(P.map, seq, (key0 + i * RPP + wave * RPW) >> P.map.shift);
         }
     };
-    auto rows_of = [&](int key0, size_t (&row)[PASSES]) {   // takes the entries, and asks for those of the next tile first: loads end in order
-        row[0] = stored_row(P, check_page(P.map, pg[0]), I.kvh, key0 + wave * RPW);
+    auto rows_of = [&](int seq, int kvh, int key0, const int (&e)[PASSES], size_t (&row)[PASSES]) {   // and asks for the entries of the next tile first: loads end in order
+        row[0] = stored_row(P, check_page(P.map, e[0]), kvh, key0 + wave * RPW);
 #pragma unroll
         for (int i = 1; i < PASSES; ++i) row[i] = row[0] + i * RPP;
         if (!whole) {
 #pragma unroll
-            for (int i = 1; i < PASSES; ++i) row[i] = stored_row(P, check_page(P.map, pg[i]), I.kvh, key0 + i * RPP + wave * RPW);
+            for (int i = 1; i < PASSES; ++i) row[i] = stored_row(P, check_page(P.map, e[i]), kvh, key0 + i * RPP + wave * RPW);
         }
-        pages(key0 + PAT_BK);
+        pages(seq, key0 + PAT_BK);
     };
     // values of V that are not finite, in a tile that some row does not see all of: staged as 0, and their rows noted
     auto note = [&](int which, int rr, bool bad) {
@@ -583,9 +610,9 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     // e4m3: through registers, which widen
     u32x4 kr[PASSES], vr[PASSES];
     uint32_t ksr[PASSES], vsr[PASSES];
-    auto load_codes = [&](int key0) {
+    auto load_codes = [&](int seq, int kvh, int key0, const int (&e)[PASSES]) {
         size_t row[PASSES];
-        rows_of(key0, row);
+        rows_of(seq, kvh, key0, e, row);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             kr[i] = *(const u32x4*)((const uint8_t*)P.k + row[i] * D + lane * 16);
@@ -594,7 +621,7 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
             vsr[i] = (P.vs + row[i])[lrow];
         }
     };
-    auto stage_codes = [&](int key0, int which) {
+    auto stage_codes = [&](int key0, int which, int lim0, int k1) {
         T *bk = (T*)lds + which * BUF, *bv = bk + PAT_BK * D;
         const bool masked = key0 + PAT_BK - 1 > lim0;
 #pragma unroll
@@ -612,9 +639,9 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
         }
     };
     // 16-bit rows: straight into LDS, a lane's place fixed, so the lane fetches the chunk that belongs there
-    auto fetch = [&](int key0, int which) {
+    auto fetch = [&](int seq, int kvh, int key0, const int (&e)[PASSES], int which) {
         size_t row[PASSES];
-        rows_of(key0, row);
+        rows_of(seq, kvh, key0, e, row);
         const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds + which * (BUF * 2);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
@@ -726,60 +753,104 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
     };
 
     if (k0 < k1) {
-        pages(k0);
-        if constexpr (Q8) { load_codes(k0); stage_codes(k0, 0); }
-        else fetch(k0, 0);
+        pages(I.seq, k0);
+        if constexpr (Q8) { load_codes(I.seq, I.kvh, k0, pg); stage_codes(k0, 0, lim0, k1); }
+        else fetch(I.seq, I.kvh, k0, pg, 0);
     }
-#pragma unroll
-    for (int s = 0; s < QS; ++s) arrived(qf[s]);
     int cur = 0;
-    for (int key0 = k0; key0 < k1; key0 += PAT_BK, cur ^= 1) {
-        if constexpr (!Q8) loads_done();
-        __syncthreads();
-        const int nxt = key0 + PAT_BK;
-        if constexpr (Q8) {
-            if (nxt < k1) load_codes(nxt);
-        } else {
-            if (key0 + PAT_BK - 1 > lim0) clean(key0, cur);
-            if (nxt < k1) fetch(nxt, cur ^ 1);
+    for (bool first_unit = true;; first_unit = false) {
+        // the next unit, looked up while this one's first tile is on its way: its own first one follows this one's last
+        int nseq = I.seq, nkvh = I.kvh + 1, nsteps = steps;
+        Rows nR = {I.first, I.rows, I.past, I.end};
+        bool next = false;
+        if constexpr (SHARED) {
+            next = left > upto - from;
+            if (next && nkvh == P.h_kv) {
+                nkvh = 0;
+                do { if (++nseq == P.n_seqs) break; nR = rows_of_seq<true>(P, nseq); nsteps = steps_of(nR.end); } while (nsteps == 0);
+                next = nseq < P.n_seqs;
+            }
+            if (next) {
+                const __attribute__((address_space(4))) int32_t* const t =
+                    (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(P.map.table + (size_t)nseq * P.map.width);
+#pragma unroll
+                for (int i = 0; i < PASSES; ++i) {
+                    const int at = (i * RPP + wave * RPW) >> P.map.shift;
+                    npg[i] = t[at < P.map.width ? at : P.map.width - 1];
+                }
+            }
         }
-        if (key0 <= lim_hi) compute(key0, cur, key0 + PAT_BK - 1 > lim_lo);
-        if constexpr (Q8) {
-            if (nxt < k1) stage_codes(nxt, cur ^ 1);
+        const int nleft = left - (upto - from);
+        int nk1 = nleft < nsteps ? nleft * PAD_STEP : nR.end;
+        nk1 = nk1 < nR.end ? nk1 : nR.end;
+        m_run = -INFINITY; l_run = 0.f;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) o_acc[i] = floatx16{};
+#pragma unroll
+        for (int s = 0; s < QS; ++s) arrived(qf[s]);
+        for (int key0 = k0; key0 < k1; key0 += PAT_BK, cur ^= 1) {
+            if constexpr (!Q8) loads_done();
+            __syncthreads();
+            const int nxt = key0 + PAT_BK;
+            const bool more = nxt < k1, over = SHARED && !more && next;
+            if constexpr (Q8) {
+                if (more) load_codes(I.seq, I.kvh, nxt, pg);
+                else if (over) load_codes(nseq, nkvh, 0, npg);
+            } else {
+                if (key0 + PAT_BK - 1 > lim0) clean(key0, cur);
+                if (more) fetch(I.seq, I.kvh, nxt, pg, cur ^ 1);
+                else if (over) fetch(nseq, nkvh, 0, npg, cur ^ 1);
+            }
+            if (key0 <= lim_hi) compute(key0, cur, key0 + PAT_BK - 1 > lim_lo);
+            if constexpr (Q8) {
+                if (more) stage_codes(nxt, cur ^ 1, lim0, k1);
+                else if (over) stage_codes(0, cur ^ 1, nR.past < nk1 ? nR.past : nk1 - 1, nk1);
+            }
         }
-    }
 
-    {
-        unsigned a = __builtin_bit_cast(unsigned, l_run), c = a;
-        lane_swap32(a, c);
-        l_run = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, c);
-    }
-    if (!live) return;
-    if (I.n_parts <= 1) {
-        const float inv = l_run != 0.f ? 1.0f / l_run : 0.f;        // a row that sees nothing: zeros
-        T* dst = (T*)P.out + (size_t)(I.first + token) * P.out_stride + (size_t)head * D + 4 * h;
+        {
+            unsigned a = __builtin_bit_cast(unsigned, l_run), c = a;
+            lane_swap32(a, c);
+            l_run = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, c);
+        }
+        const bool all = SHARED ? from == 0 && upto == steps : I.n_parts <= 1;
+        if constexpr (SHARED) {
+            if (from == 0 && tid == 0)              // where the join finds the unit's parts
+                P.units[I.seq * P.h_kv + I.kvh] = int2{(int)(2 * blockIdx.x + (first_unit ? 0 : 1)), all ? 1 : 1 + (steps - upto + per - 1) / per};
+        }
+        if (live && all) {
+            const float inv = l_run != 0.f ? 1.0f / l_run : 0.f;        // a row that sees nothing: zeros
+            T* dst = (T*)P.out + (size_t)(I.first + token) * P.out_stride + (size_t)head * D + 4 * h;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v4 w;
+                for (int i = 0; i < 4; ++i) {
+                    v4 w;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (T)(o_acc[b][4 * i + j] * inv);
-                *(v4*)(dst + 32 * b + 8 * i) = w;
-            }
-    } else {
-        const size_t pr = ((size_t)I.split * P.n_rows + I.first + token) * P.n_heads + head;
-        float* dst = P.part_o + pr * D + 4 * h;
+                    for (int j = 0; j < 4; ++j) w[j] = (T)(o_acc[b][4 * i + j] * inv);
+                    *(v4*)(dst + 32 * b + 8 * i) = w;
+                }
+        } else if (live) {
+            const size_t pr = SHARED ? (size_t)(2 * blockIdx.x + (first_unit ? 0 : 1)) * P.tile_rows + r
+                                     : ((size_t)I.split * P.n_rows + I.first + token) * P.n_heads + head;
+            float* dst = P.part_o + pr * D + 4 * h;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                floatx4 w;
+                for (int i = 0; i < 4; ++i) {
+                    floatx4 w;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = o_acc[b][4 * i + j];
-                *(floatx4*)(dst + 32 * b + 8 * i) = w;
-            }
-        if (h == 0) { P.part_ml[pr * 2] = m_run; P.part_ml[pr * 2 + 1] = l_run; }
+                    for (int j = 0; j < 4; ++j) w[j] = o_acc[b][4 * i + j];
+                    *(floatx4*)(dst + 32 * b + 8 * i) = w;
+                }
+            if (h == 0) { P.part_ml[pr * 2] = m_run; P.part_ml[pr * 2 + 1] = l_run; }
+        }
+        if (!next) return;
+        left = nleft; from = 0; steps = nsteps;
+        I.seq = nseq; I.kvh = nkvh; I.first = nR.first; I.past = nR.past; I.end = nR.end;
+        I.rows = nR.rows < P.tile_rows ? nR.rows : P.tile_rows;
+        at_unit();
+        enter();
     }
 }
 
@@ -828,10 +899,10 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(PagedAttnPara
     }
 }
 
-// Joins what the workgroups of paged_attention_rows_kernel left of a unit: NW waves a (row, head), each takes every NWth part, eight
+// Joins what the workgroups that share all units' keys left of a unit: NW waves a (row, head), each takes every NWth part, eight
 // of them in flight at once.  A unit's first part lies where the workgroup that began it said, the others at the first place of
 // the workgroups behind it.
-template <typename T, int D, int ROWS, int NW>
+template <typename T, int D, int NW>
 __global__ void __launch_bounds__(256) paged_attention_join_rows_kernel(PagedAttnParams P) {
     constexpr int E = D / 64, MAX = 8;                      // outputs a lane, parts a wave at a time
     typedef float vecE __attribute__((ext_vector_type(E)));
@@ -842,13 +913,13 @@ __global__ void __launch_bounds__(256) paged_attention_join_rows_kernel(PagedAtt
     const int seq = t < P.n_rows ? __builtin_amdgcn_readfirstlane(seq_of_row(P.cu_rows, P.n_seqs, t)) : P.n_seqs;
     if (seq >= P.n_seqs) return;                            // (NW > 1: the whole block's row)
     const int first = P.cu_rows[seq], n = P.cu_rows[seq + 1] - first, r = (t - first) * P.group + head % P.group;
-    if (first < 0 || n > P.n_rows - first || r < 0 || r >= ROWS) return;       // rows that were left out
+    if (first < 0 || n > P.n_rows - first || r < 0 || r >= P.tile_rows) return;       // rows that were left out
     const int2 u = P.units[seq * P.h_kv + head / P.group];
     // a unit without keys (a length below zero) has no parts, and nobody wrote its entry: its rows are zeros
-    const bool none = attn_tile_end(P, P.seq_lens[seq], n * P.group, 0, ROWS) == 0;
+    const bool none = attn_tile_end(P, P.seq_lens[seq], n * P.group, 0, P.tile_rows) == 0;
     const int parts = __builtin_amdgcn_readfirstlane(none ? 0 : u.y), g0 = __builtin_amdgcn_readfirstlane(u.x);
     if (parts == 1) return;                                 // written already
-    auto slot = [&](int p) { return (size_t)(p ? (g0 & ~1) + 2 * p : g0) * ROWS + r; };
+    auto slot = [&](int p) { return (size_t)(p ? (g0 & ~1) + 2 * p : g0) * P.tile_rows + r; };
     float top = -INFINITY;
     for (int p = lane; p < parts; p += 64) top = fmaxf(top, P.part_ml[slot(p) * 2]);
     vecE mine = {};
@@ -893,8 +964,11 @@ static AttnPlan attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int
     const int64_t rows = (int64_t)max_rows * (n_heads / h_kv), units = (int64_t)n_seqs * h_kv;
     A.n_tiles = A.n_splits = 1;
     A.split_len = max_len;
-    if (rows <= 32) {
-        A.tile_rows = rows <= 16 ? 16 : 32;
+    // Shared evenly: few rows always; up to a tile of them where the units are neither few, whose keys the split below divides evenly
+    // enough, nor as many as fit the card, which need no split.  Shared | split, six tokens of 64 / 8 heads over 300-4000 fp16 keys: 64
+    // units 27.7 | 27.2 us, 128 39.5 | 45.3, 256 77 | 83, 384 of 2000 keys 99 | 118, 512 149 | 134, 768 175 | 154.
+    if (rows <= 32 || (rows <= 128 && max_len > 256 && units >= 128 && units < 512)) {
+        A.tile_rows = rows <= 16 ? 16 : (int)((rows + 31) / 32 * 32);
         // as many workgroups as fit the card (256 CUs; by registers and LDS), but none for fewer than 256 keys
         const int64_t fit = 256 * 2, most = units * ((max_len + 255) / 256);
         A.n_groups = max_len <= 256 ? 0 : (int)(fit < most ? fit : most);
@@ -950,16 +1024,17 @@ extern "C" int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t 
 #define SQ_KERNELS(TT, DD, QQ) do { \
         if (A.tile_rows == 16) SQ_LAUNCH((paged_attention_rows_kernel<TT, DD, QQ, 1>), grid, P); \
         else if (A.tile_rows == 32) SQ_LAUNCH((paged_attention_rows_kernel<TT, DD, QQ, 2>), grid, P); \
-        else SQ_LAUNCH((paged_attention_tiles_kernel<TT, DD, QQ>), grid, P); \
+        else if (A.n_groups) SQ_LAUNCH((paged_attention_tiles_kernel<TT, DD, QQ, true>), grid, P); \
+        else SQ_LAUNCH((paged_attention_tiles_kernel<TT, DD, QQ, false>), grid, P); \
     } while (0)
     // the join of few rows gives each four waves (a part of the key axis each at a time), of many one
-#define SQ_JOIN_ROWS(TT, DD, RR) do { \
-        if (join < 1024) SQ_LAUNCH((paged_attention_join_rows_kernel<TT, DD, RR, 4>), join, P); \
-        else SQ_LAUNCH((paged_attention_join_rows_kernel<TT, DD, RR, 1>), (join + 3) / 4, P); \
+#define SQ_JOIN_ROWS(TT, DD) do { \
+        if (join < 1024) SQ_LAUNCH((paged_attention_join_rows_kernel<TT, DD, 4>), join, P); \
+        else SQ_LAUNCH((paged_attention_join_rows_kernel<TT, DD, 1>), (join + 3) / 4, P); \
     } while (0)
 #define SQ_TYPES(TT, DD) do { \
         if (k_scales) SQ_KERNELS(TT, DD, true); else SQ_KERNELS(TT, DD, false); \
-        if (A.n_groups) { if (A.tile_rows == 16) SQ_JOIN_ROWS(TT, DD, 16); else SQ_JOIN_ROWS(TT, DD, 32); } \
+        if (A.n_groups) SQ_JOIN_ROWS(TT, DD); \
         else if (A.n_splits > 1) SQ_LAUNCH((paged_attention_join_kernel<TT, DD>), join, P, A.tile_rows); \
     } while (0)
     if (dtype == SQ_DTYPE_F16) { if (d == 128) SQ_TYPES(half_t, 128); else SQ_TYPES(half_t, 64); }

@@ -91,6 +91,15 @@ def test_workspace_of_the_attention():
                         assert left == 0 and parts <= 64 and parts != 1 and (parts == 0 or max_len > 512 * (parts - 1))
 
 
+def test_attention_workspace_of_a_few_tokens_of_shared_heads():
+    """33 to 128 rows: two parts of a tile's rows a workgroup where the keys are shared out, nothing where every unit has its own."""
+    lib = native.load()
+    size = lambda seqs, rows, length: lib.sq_paged_attention_workspace_bytes(seqs, seqs * rows, rows, length, 64, 8, 128)
+    for rows, tile in ((5, 64), (8, 64), (9, 96), (16, 128)):
+        assert size(32, rows, 5000) == 512 * 2 * tile * 130 * 4 + 256 * 8
+        assert size(64, rows, 5000) == size(32, rows, 256) == 0
+
+
 def test_front_end_refuses_host_tensors():
     from sequoia_amd.ops import HipOps
     ops = HipOps()

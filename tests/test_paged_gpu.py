@@ -372,6 +372,37 @@ def test_attention_with_offsets_that_name_no_rows(ops, heads, h_kv, most):
         assert bool(((got[:1].double() - want).abs() <= bound).all())                 # the first row is there whatever the bound
 
 
+@pytest.mark.parametrize("dtype,quantised", [(torch.float16, False), (torch.bfloat16, False), (torch.float16, True), (torch.bfloat16, True)])
+@pytest.mark.parametrize("heads,h_kv,d,page,past,new", [
+    (64, 8, 128, 64, [300, 1900, 0, 64, 63, 700, 5, 1100] * 2, [5, 6, 5, 1, 6, 0, 8, 7] * 2),       # 33 to 64 rows of shared heads
+    (64, 8, 128, 64, [300, 1900, 0, 64], [5, 6, 5, 8]),                                             # (few units)
+    (8, 1, 64, 16, [1000, 31, 250, 200] * 35, [12, 11, 1, 9] * 35),                                 # to 96, pages shorter than a tile
+    (32, 2, 128, 32, [500, 800] * 33, [8, 7] * 33),                                                 # 128, all of a tile
+    (12, 12, 64, 256, [900, 2000, 130] * 4, [40, 33, 100] * 4),                                     # no sharing
+    (16, 2, 128, 128, [1500, 0] * 35, [7, 5] * 35),
+])
+def test_attention_of_a_few_tokens_of_shared_heads(ops, heads, h_kv, d, page, past, new, dtype, quantised):
+    """33 to 128 rows a sequence and KV head: the keys of between 128 and 512 such units are shared out evenly too."""
+    pool = Pool([p + n for p, n in zip(past, new)], h_kv, d, page, dtype, quantised, 31)
+    q = torch.randn((heads, sum(new) + 2, d), generator=torch.Generator().manual_seed(6)).to(dtype)
+    for bounds in (dict(max_rows=max(new), max_len=max(p + n for p, n in zip(past, new))), dict(max_rows=max(new))):
+        check_attention(pool, q, run_attention(ops, pool, q.to(DEV), past, new, d ** -0.5, 2, **bounds), past, new, d ** -0.5)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_attention_of_many_sequences_with_shared_heads(ops, quantised):
+    """Units of every length, none among them, fewer and more than the workgroups that fit the card."""
+    rng = __import__("random").Random(7)
+    n, heads, h_kv, d, dtype = 110 if quantised else 150, 24, 4, 64, torch.float16
+    new = [rng.randint(0, 9) for _ in range(n)]
+    past = [rng.choice((0, rng.randint(0, 70), rng.randint(200, 900))) for _ in range(n)]
+    new[0] = new[-1] = 0
+    pool = Pool([p + m for p, m in zip(past, new)], h_kv, d, 64, dtype, quantised, 33)
+    q = torch.randn((heads, sum(new) + 3, d), generator=torch.Generator().manual_seed(2)).to(dtype)
+    out = run_attention(ops, pool, q.to(DEV), past, new, d ** -0.5, 3, max_rows=9, max_len=max(p + m for p, m in zip(past, new)))
+    check_attention(pool, q, out, past, new, d ** -0.5)
+
+
 @pytest.mark.parametrize("heads,h_kv,new", [(4, 4, 3), (8, 1, 2), (2, 2, 40)])
 def test_attention_of_a_length_below_zero(ops, heads, h_kv, new):
     """Rows that see nothing are zeros, also where a whole sequence has no key and its neighbours are split."""
@@ -447,6 +478,34 @@ def test_attention_what_a_row_does_not_see_does_not_reach_it(ops, heads, h_kv, d
         assert torch.equal(got[t:t + s], clean[t:t + s])
         assert bool(got[t + s:t + n].isnan().view(n - s, -1).any(-1).all())
         t += n
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_attention_of_shared_keys_keeps_hidden_rows_apart(ops, quantised):
+    """The same where many sequences' keys are shared out over the workgroups: behind every sequence's end, and in its last token, which
+    the others of its chunk do not see."""
+    heads, h_kv, d, page, dtype, past, new = 16, 2, 64, 32, torch.float16, [3, 300, 61, 127] * 17, [6, 5, 3, 8] * 17
+    total = [p + n for p, n in zip(past, new)]
+    pool = Pool(total, h_kv, d, page, dtype, quantised, 43, width=max(-(-t // page) for t in total) + 1)
+    q = torch.randn((heads, sum(new), d), generator=torch.Generator().manual_seed(5)).to(dtype).to(DEV)
+    kw = dict(max_rows=max(new), max_len=max(total))
+    clean = run_attention(ops, pool, q, past, new, d ** -0.5, **kw)
+    check_attention(pool, q.cpu(), clean, past, new, d ** -0.5)
+    last = torch.tensor([sum(new[:b + 1]) - 1 for b in range(len(new))])
+    before = torch.ones(sum(new), dtype=torch.bool)
+    before[last] = False
+    for back in (0, 1):                                      # from the end on, from the last token on
+        for which in (0, 1):
+            t = pool.pages[which].clone().view(torch.uint8) if quantised else pool.pages[which].clone()
+            for b in range(len(total)):
+                for j in range(total[b] - back, min(total[b] + 40, pool.width * page)):
+                    t[int(pool.table[b, j // page]), :, j % page, ::5] = 0x7f if quantised else (math.inf if which else math.nan)
+            pool.dev[which] = t.to(DEV).view(torch.float8_e4m3fn) if quantised else t.to(DEV)
+        got = run_attention(ops, pool, q, past, new, d ** -0.5, **kw)
+        if back == 0:
+            assert torch.equal(got, clean)
+        else:
+            assert torch.equal(got[before], clean[before]) and not bool(got[last].isfinite().all(-1).any())
 
 
 def test_attention_hidden_infinite_value_stays_an_infinity_where_it_is_seen(ops):
