@@ -586,7 +586,7 @@ def test_attention_bounds_that_cut_and_bad_pages(ops):
     assert bool(((bad[10:].view(10, heads, d).double() - want).abs() <= bound).all()) and bool(good.isfinite().all())
 
 
-@pytest.mark.parametrize("past,new,heads", [([4000, 77], [1, 1], 8), ([300], [40], 8)])
+@pytest.mark.parametrize("past,new,heads", [([4000, 77], [1, 1], 8), ([300], [40], 8), ([900, 150, 20, 400] * 17, [11, 5, 9, 10] * 17, 8)])
 def test_attention_replays_in_a_graph_with_other_lengths(ops, past, new, heads):
     """One captured launch serves every step whose bounds hold: lengths, tables and rows are read on the device; several replays
     with eager work between them, each against the eager result."""
