@@ -19,6 +19,7 @@ from ..ops import get_ops
 from .Llama_KV import KV_Cache
 from .Llama_model import KVConfigView, LlamaForCausalLM_FI, LlamaForCausalLM_TG, load_weights
 from .Llama_modules import TreeContext
+from .ts_linear import capture_mode
 
 
 class InferenceEngine:
@@ -95,7 +96,7 @@ def prime_graph_rng(device):
         s = torch.cuda.Stream(device=device)
         s.wait_stream(torch.cuda.current_stream(device))
         with torch.cuda.stream(s):
-            with torch.cuda.graph(g, stream=s):
+            with torch.cuda.graph(g, stream=s, capture_error_mode=capture_mode()):
                 pass
         torch.cuda.current_stream(device).wait_stream(s)
     _PRIMED[key] = g
@@ -133,7 +134,7 @@ class _GraphRunner:
         torch.cuda.current_stream().wait_stream(s)
         self.graph = torch.cuda.CUDAGraph()
         kv.kv_offset = 0
-        with torch.cuda.graph(self.graph, pool=mempool):
+        with torch.cuda.graph(self.graph, pool=mempool, capture_error_mode=capture_mode()):
             self.logits = self._run()
         kv.kv_offset, kv.dirty_end = saved
 

@@ -27,6 +27,13 @@ import torch.nn.functional as F
 
 from ..ops import get_ops
 
+
+def capture_mode():
+    """capture_error_mode of this package's graph captures.  With a process group alive its watchdog thread queries the events of
+    earlier collectives whenever it wakes; a capture that watches all threads makes such a query an error that ends the process."""
+    dist = torch.distributed
+    return "thread_local" if dist.is_available() and dist.is_initialized() else "global"
+
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PLAN_FILE = os.path.join(_PKG, "ts_plans_gfx950.json")
 MAX_ROWS = 144
@@ -284,7 +291,7 @@ class TsLinearSet:
                     fn(i % n_layers)
                 side.synchronize()
                 g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, stream=side):
+                with torch.cuda.graph(g, stream=side, capture_error_mode=capture_mode()):
                     for i in range(reps):
                         fn(i % n_layers)
                 g.replay()

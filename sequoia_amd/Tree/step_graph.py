@@ -17,6 +17,7 @@ import torch
 
 from ..Engine.Llama_modules import TreeContext
 from ..Engine.ts_linear import MAX_ROWS as TS_MAX_ROWS
+from ..Engine.ts_linear import capture_mode
 from ..native import (SQ_RES_N_TREE, SQ_RESULT_INTS, SQ_RESULT_RING, SQ_STEP_ACTIVE, SQ_STEP_GT, SQ_STEP_INTS,
                       SQ_VERIFY_GATHER_FIRST)
 from ..ops import get_ops
@@ -230,7 +231,7 @@ class StepState:
         self.step[SQ_STEP_GT] = 1
         graph = torch.cuda.CUDAGraph()
         kw = dict(stream=torch.cuda.Stream(device=self.device, priority=-1)) if OVERLAP_LAST_LEVEL == "2" else {}
-        with torch.cuda.graph(graph, **kw):
+        with torch.cuda.graph(graph, capture_error_mode=capture_mode(), **kw):
             self.body()
         self.graph = graph
         for kv, off, dirty in marks:
