@@ -979,11 +979,14 @@ static AttnPlan attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int
     A.tile_rows = 128;
     A.n_tiles = (int)((rows + 127) / 128);
     // Few tiles: the key axis is split for one round of the two workgroups that share a CU, in parts of 512 keys or more.  Parts are
-    // dear here, 128 rows of fp32 sums each: with four rounds in parts of 256, 2048 rows of 32 heads took 157 us instead of 59.
+    // dear here, 128 rows of fp32 sums each: with four rounds in parts of 256, 2048 rows of 32 heads took 157 us instead of 59.  Parts of
+    // 256 keys where there are hardly any tiles: six tokens of 64 / 8 heads behind 1000 keys 12.7 instead of 17.0 us, behind 8000
+    // 15.2 instead of 18.0; with 64 tiles 37.9 instead of 36.1; parts of 128 take longer from 8000 keys on (17.3).
     int64_t want = (512 + units * A.n_tiles - 1) / (units * A.n_tiles);
     want = want > 64 ? 64 : want;
     int64_t len = (max_len + want - 1) / want;
-    len = len < 512 ? 512 : len;
+    const int64_t least = units * A.n_tiles <= 32 ? 256 : 512;
+    len = len < least ? least : len;
     A.split_len = (int)((len + 127) / 128 * 128);
     A.n_splits = (max_len + A.split_len - 1) / A.split_len;
     if (A.n_splits > 1) A.bytes = (A.parts = (size_t)A.n_splits * n_rows * n_heads) * (d + 2) * sizeof(float);

@@ -88,7 +88,7 @@ def test_workspace_of_the_attention():
                         assert left == 0 and 1 <= groups <= 512 and groups <= n_seqs * kv * -(-max_len // 256)
                     else:
                         parts, left = divmod(got, rows * heads * 130 * 4)
-                        assert left == 0 and parts <= 64 and parts != 1 and (parts == 0 or max_len > 512 * (parts - 1))
+                        assert left == 0 and parts <= 64 and parts != 1 and (parts == 0 or max_len > 256 * (parts - 1))
 
 
 def test_attention_workspace_of_a_few_tokens_of_shared_heads():
