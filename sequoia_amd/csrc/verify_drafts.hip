@@ -10,10 +10,10 @@
 // the token in it.  The first reads every logit once; the others touch two rows a sequence and are bound by the latency of their
 // chains of loads, so that neither has a barrier.  (The draw in the second launch's last workgroup of a sequence: every workgroup's
 // release writes its XCD's L2 back, and the two launches' time grew by a third.)
-// One sequence of five drafted tokens, 32000 tokens, fp16: 11.8 us on the device.  64 sequences of 0-8: 31.5 us, 19 of it the first
-// launch, bound by the vector ALU -- 20 instructions a logit, of which 16 are 64-bit; every one of them takes four
+// One sequence of five drafted tokens, 32000 tokens, fp16: 11.8 us on the device.  64 sequences of 0-8: 31.9 us, 19 of it the first
+// launch, bound by the vector ALU -- 21 instructions a logit, of which 17 are 64-bit; every one of them takes four
 // cycles and a little, 64-bit or not -- and not by the 5.1 TB/s that its bytes would allow.  24 sequences of 2-6 with 128261 tokens,
-// bf16: 42 us, 28 of it the first launch.
+// bf16: 43 us, 28 of it the first launch.
 #include "paged.h"
 
 #define VD_THREADS 256
@@ -46,9 +46,9 @@ struct VerifyDraftsParams {
 __device__ __forceinline__ double log2e_over(float t) {
     return t > 0.f ? 1.4426950408889634 / (double)(t < 1e30f ? t : 1e30f) : 0.0;
 }
-// e^((x - top) / T) with c = log2(e) / T, x <= top: 2^t, t = (x - top) c, to 4e-14 (NaN stays).  t = k + f, |f| <= 1/2, and
-// 2^f = 1 + f g(f) with g of degree 8, interpolated at the Chebyshev nodes; the weight of the maximum is exactly 1.  t stops at
-// -1080, where the result is 0.
+// e^((x - top) / T) with c = log2(e) / T, x <= top: 2^t, t = (x - top) c, to 4e-14, and |t| 2^-53 from t's own rounding (NaN
+// stays).  t = k + f, |f| <= 1/2, and 2^f = 1 + f g(f) with g of degree 8, interpolated at the Chebyshev nodes; the weight of the
+// maximum is exactly 1.  t stops at -1080, where the result is 0.
 struct Exp2 {
     double g[9];
     __device__ __forceinline__ Exp2()
@@ -75,11 +75,13 @@ __device__ __forceinline__ double weight(const Exp2& E, double x, double top, do
     const double g = exp2_parts(E, t, k);
     return __builtin_amdgcn_ldexp(g, (int)k);
 }
-// The sum of eight of them beside a sum that holds a 1 already, in two thirds of the instructions (they bound the first launch): t
-// by one fused operation from shift = -top c, whose rounding is one factor for the whole sum; a stop at -1020, which no sum beside
-// a 1 notices, so that k goes straight into the exponent's bits.  Four at a time: one alone is a chain of dependent instructions.
+// The sum of eight of them beside a sum that holds a 1 already, in fewer instructions (they bound the first launch): a stop at -1020,
+// which no sum beside a 1 notices, so that k goes straight into the exponent's bits.  Four at a time: one alone is a chain of
+// dependent instructions.  x - top comes before the factor, as in weight(): x c - top c in one fused operation saves an instruction
+// (31.5 | 31.9 us for 64 sequences) but is off by the rounding of top c, which the other side of a comparison does not have: 1e-15 of
+// the sum at ordinary temperatures, enough to accept what ties, 2e-7 at T = 1e-8, a factor of 4 at 1e-15, and no number at all below.
 // Not for NaN.
-__device__ __forceinline__ double weights_in_sum(const Exp2& E, const float (&x)[8], double shift, double c) {
+__device__ __forceinline__ double weights_in_sum(const Exp2& E, const float (&x)[8], double top, double c) {
     const double big = 6755399441055744.0;
     double sum = 0.0;
 #pragma unroll
@@ -87,7 +89,7 @@ __device__ __forceinline__ double weights_in_sum(const Exp2& E, const float (&x)
         double f[4], g[4];
         uint32_t k[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = __builtin_fmax(__builtin_fma((double)x[h + j], c, shift), -1020.0);
+        for (int j = 0; j < 4; ++j) f[j] = __builtin_fmax(((double)x[h + j] - top) * c, -1020.0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const double kb = f[j] + big;
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(VD_THREADS, 6) verify_drafts_stats_kernel(Veri
     const Exp2 E;
     float top = -INFINITY, best = -INFINITY;
     int first = 0x7fffffff;
-    double sum = 0.0, shift = 0.0;
+    double sum = 0.0;
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
@@ -233,10 +235,9 @@ __global__ void __launch_bounds__(VD_THREADS, 6) verify_drafts_stats_kernel(Veri
             if (__any(m > top)) {                            // (seldom, after a row's first chunks)
                 m = wave_max_f32_dpp(m);
                 if (top > -INFINITY) sum *= weight(E, (double)top, (double)m, c);
-                shift = -(double)m * c;
                 top = m;
             }
-            if (top > -INFINITY) sum += weights_in_sum(E, x, shift, c);       // else nothing so far counts
+            if (top > -INFINITY) sum += weights_in_sum(E, x, (double)top, c);       // else nothing so far counts
         } else {                                             // greedy: the first maximum
 #pragma unroll
             for (int j = 0; j < 8; ++j)
