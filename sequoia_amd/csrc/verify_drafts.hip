@@ -42,9 +42,9 @@ struct VerifyDraftsParams {
     float* token_logit;      // [rows of stats]: the logit of the drafted token that the row judges, or was drawn from
 };
 
-// log2(e) / T; 0: greedy.  1e30 is as flat as any temperature above it
+// log2(e) / T; 0: greedy.  An infinite T is the largest finite one (0 would be greedy)
 __device__ __forceinline__ double log2e_over(float t) {
-    return t > 0.f ? 1.4426950408889634 / (double)(t < 1e30f ? t : 1e30f) : 0.0;
+    return t > 0.f ? 1.4426950408889634 / (double)fminf(t, 0x1.fffffep127f) : 0.0;
 }
 // e^((x - top) / T) with c = log2(e) / T, x <= top: 2^t, t = (x - top) c, to 4e-14, and |t| 2^-53 from t's own rounding (NaN
 // stays).  t = k + f, |f| <= 1/2, and 2^f = 1 + f g(f) with g of degree 8, interpolated at the Chebyshev nodes; the weight of the

@@ -99,3 +99,20 @@ def test_any_temperature_matches_the_definition(ops, temperature, dtype):
 @pytest.mark.parametrize("offset,temperature", LARGE)
 def test_large_logits_match_the_definition(ops, offset, temperature):
     check(ops, with_plateaus([3, 0, 2, 5, 1, 4, 4, 2], 9000, torch.float32, 73, offset), temperature)
+
+
+@pytest.mark.parametrize("temperature", [1e31, 1e34, 3e38])
+def test_large_logits_at_large_temperatures(ops, temperature):
+    """Steps of fp32 near 3e38 are 2e31 wide: the same order as these temperatures, or far under them."""
+    check(ops, with_plateaus([3, 0, 2, 5, 1, 4, 4, 2], 9000, torch.float32, 74, 3e38), temperature)
+    inputs = case([3, 0, 2, 5], 5000, torch.float32, 75)
+    check(ops, (3e37 * inputs[0], 3e37 * inputs[1], *inputs[2:]), temperature)
+
+
+def test_an_infinite_temperature_is_flat(ops):
+    """Every token above -inf has the same mass."""
+    t, d, tok, cu, ua, un = case([0, 0], 4000, torch.float16, 76)
+    t[:, ::3] = -math.inf
+    left = [i for i in range(4000) if i % 3]
+    want = [left[int(float(u) * len(left))] for u in un]
+    assert run(ops, t, d, tok, cu, ua, un, [math.inf, 1.0e38]) == ([0, 0], want)
