@@ -2,7 +2,7 @@
 // stored rows and n new ones, row i attends keys [0, past + i],
 //     o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   s_j = scale * q . k_j,
 // in one pass over the keys with a running maximum and sum in fp32; weights are rounded to the element type once, for the
-// second matrix product.  The query heads that share a KV head are packed into the same rows of a tile (row r = token r / group,
+// second matrix product, and the sum is taken of the rounded ones.  The query heads that share a KV head are packed into the same rows of a tile (row r = token r / group,
 // head r % group), so that every stored row is read once for all of them.
 #include "paged.h"
 #include "attn_map.h"
@@ -392,14 +392,9 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
                     for (int nt = 0; nt < NT; ++nt) o_acc[mt][nt] *= alpha;
                     m_run[mt] = m_new;
                 }
-                float psum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float p = __builtin_amdgcn_exp2f(sv[j] - m_use);
-                    psum += p;
-                    pf[mt][j] = (T)p;
-                }
-                l_run[mt] += psum;
+                for (int j = 0; j < 8; ++j) pf[mt][j] = (T)__builtin_amdgcn_exp2f(sv[j] - m_use);
+                l_run[mt] = add_weights<T>(pf[mt], l_run[mt]);
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
