@@ -56,6 +56,11 @@ template <typename T> __device__ __forceinline__ float add_weights(typename vec_
     return c + d;
 }
 
+// log2 of what weights are multiplied by before they are rounded for the second product, numerator and denominator alike, with
+// `headroom` doublings left: fp16 ends at 2^16 and loses bits below 2^-14.  From 1 down, the weights of a long context under one key
+// that stands out would be among those: 100000 of e^-17 are a 250th of the row, and each of them less than half of the smallest step.
+template <typename T> constexpr float weight_shift(int headroom) { return __is_same(T, half_t) ? (float)(15 - headroom) : 0.f; }
+
 // column (lane & 15) of the 4 x 16 block of 16-bit values whose row (lane & 15) >> 2, columns 4 (lane & 3).. this lane addresses
 __device__ __forceinline__ u32x2 read_transposed(const void* p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)p));
@@ -384,14 +389,15 @@ __global__ void __launch_bounds__(PAD_NW * 64, 2) paged_attention_rows_kernel(Pa
                 for (int j = 0; j < 8; ++j) cmax = fmaxf(cmax, sv[j]);
                 cmax = group4_max(cmax);
                 const float m_new = fmaxf(m_run[mt], cmax);
-                const float m_use = m_new == -INFINITY ? 0.f : m_new;       // nothing seen so far
+                const float m_fin = m_new == -INFINITY ? 0.f : m_new;       // nothing seen so far
                 if (__any(m_new > m_run[mt])) {
-                    const float alpha = __builtin_amdgcn_exp2f(m_run[mt] - m_use);
+                    const float alpha = __builtin_amdgcn_exp2f(m_run[mt] - m_fin);
                     l_run[mt] *= alpha;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) o_acc[mt][nt] *= alpha;
                     m_run[mt] = m_new;
                 }
+                const float m_use = m_fin - weight_shift<T>(0);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) pf[mt][j] = (T)__builtin_amdgcn_exp2f(sv[j] - m_use);
                 l_run[mt] = add_weights<T>(pf[mt], l_run[mt]);
@@ -709,7 +715,7 @@ __global__ void __launch_bounds__(PAT_NW * 64, 2) paged_attention_tiles_kernel(P
                 for (int i = 0; i < 16; ++i) o_acc[b][i] *= alpha;
             m_run = m_new;
         }
-        const float m_use = m_run == -INFINITY ? 0.f : m_run;
+        const float m_use = (m_run == -INFINITY ? 0.f : m_run) - weight_shift<T>(8);       // (weights reach 2^8 times the maximum's)
         v8 pf[KS];
 #pragma unroll
         for (int b = 0; b < 2; ++b)

@@ -95,3 +95,26 @@ def test_what_all_values_have_in_common_comes_back_whole(ops, heads, h_kv, d, pa
     q = torch.randn((heads, sum(new), d), generator=g).to(dtype)
     out = run_attention(ops, pool, q.to(DEV), past, new, d ** -0.5, max_rows=max(new), max_len=max(total))
     check(pool, q, out, past, new, d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("above", [8.0, 17.0, 20.0])
+@pytest.mark.parametrize("heads,h_kv,d,page,past,new", [(8, 8, 64, 64, [6000], [1]), (4, 2, 128, 16, [150, 4000], [3, 2]), (8, 1, 64, 64, [5000], [9]),
+                                                        (4, 4, 64, 64, [3000], [140]), (32, 4, 64, 64, [(41 * i) % 700 + 300 for i in range(34)], [5] * 34)])
+def test_many_small_weights_beside_a_large_one(ops, heads, h_kv, d, page, past, new, above, dtype):
+    """The first key of every sequence stands out by `above` (e^17 = 2^24.5) and has a value of 0: what comes back is the others' share, all
+    of it."""
+    total = [p + n for p, n in zip(past, new)]
+    pool = Pool(total, h_kv, d, page, dtype, False, 83)
+    pool.pages[0] = torch.zeros_like(pool.pages[0])
+    pool.pages[1] = torch.ones_like(pool.pages[1])
+    for b in range(len(past)):
+        first = int(pool.table[b, 0])
+        pool.pages[0][first, :, 0, 0] = above
+        pool.pages[1][first, :, 0] = 0.0
+    pool.dev = [t.to(DEV) for t in pool.pages]
+    q = torch.zeros((heads, sum(new), d))
+    q[:, :, 0] = 1.0
+    q = q.to(dtype)
+    out = run_attention(ops, pool, q.to(DEV), past, new, 1.0, max_rows=max(new), max_len=max(total))
+    check(pool, q, out, past, new, 1.0)
