@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import importlib.util
+import json
 import os
 import shutil
 import subprocess
@@ -21,8 +22,8 @@ if PROBES:
     SOURCES = SOURCES + ["ts_probe.hip", "draft_fused.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wno-unused-value",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + (["-DSEQUOIA_BUILD_PROBES"] if PROBES else [])
-# (-packed-fp32-ops: no v_pk_{add,mul,fma}_f32 -- some of their forms have given wrong results now and then; the host pass warns that
-# it does not know the feature)
+# (-packed-fp32-ops: no v_pk_{add,mul,fma}_f32, some of whose forms can give wrong results on this hardware now and then, which no
+# test here shows reliably; the host pass warns that it does not know the feature)
 # per-source additions.  ts_linear: keep the MFMA accumulators in VGPRs -- with the AGPR form the register
 # allocator permutes the 48-128 accumulator registers on every trip of the ring loop (72 v_accvgpr_* moves
 # per 48 MFMAs in the ISA)
@@ -36,27 +37,50 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (need ROCm)")
 
 
-def _stale(target: str, deps: list[str]) -> bool:
-    if not os.path.exists(target):
+# what each built file was made of beside its sources: flags, not paths, so that a copy of the tree elsewhere is not made again
+MADE_WITH = "made_with.json"
+
+
+def _made_with() -> dict:
+    try:
+        with open(os.path.join(LIBDIR, MADE_WITH)) as f:
+            return json.load(f)
+    except (OSError, ValueError):
+        return {}
+
+
+def _stale(target: str, deps: list[str], flags: list[str]) -> bool:
+    if not os.path.exists(target) or _made_with().get(os.path.basename(target)) != flags:
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _make(target: str, cmd: list[str], flags: list[str], verbose: bool):
+    """Runs `cmd`, then notes `flags`: a build that ends early leaves nothing that passes for made."""
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    made = _made_with()
+    made[os.path.basename(target)] = flags
+    with open(os.path.join(LIBDIR, MADE_WITH), "w") as f:
+        json.dump(made, f, indent=1)
+
+
 # the paged operators' binding to torch tensors: host code, against the headers of the torch that is installed
 BINDING = os.path.join(LIBDIR, "_paged.so")
 BINDING_SOURCE = os.path.join(CSRC, "paged_binding.cpp")
+BINDING_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared"]
 
 
 def build_binding(force: bool = False, verbose: bool = True) -> str:
     torch = os.path.dirname(importlib.util.find_spec("torch").origin)
-    if force or _stale(BINDING, [BINDING_SOURCE, os.path.join(os.path.dirname(PKG), "include", "sequoia_hip.h"), os.path.join(torch, "version.py")]):
-        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-isystem", os.path.join(torch, "include"),
+    deps = [BINDING_SOURCE, os.path.join(os.path.dirname(PKG), "include", "sequoia_hip.h"), os.path.join(torch, "version.py")]
+    if force or _stale(BINDING, deps, BINDING_FLAGS):
+        cmd = [os.environ.get("CXX", "g++")] + BINDING_FLAGS + ["-isystem", os.path.join(torch, "include"),
                "-isystem", os.path.join(torch, "include", "torch", "csrc", "api", "include"), "-isystem", sysconfig.get_paths()["include"],
                BINDING_SOURCE, "-o", BINDING, "-L" + os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.check_call(cmd)
+        _make(BINDING, cmd, BINDING_FLAGS, verbose)
     return BINDING
 
 
@@ -68,17 +92,13 @@ def build(force: bool = False, verbose: bool = True) -> str:
     cc = hipcc()
     for s in srcs:
         o = os.path.join(LIBDIR, os.path.basename(s).replace(".hip", ".o"))
-        if force or _stale(o, [s] + hdrs):
-            cmd = [cc] + FLAGS + EXTRA_FLAGS.get(os.path.basename(s), []) + ["-c", s, "-o", o]
-            if verbose:
-                print(" ".join(cmd), flush=True)
-            subprocess.check_call(cmd)
+        flags = FLAGS + EXTRA_FLAGS.get(os.path.basename(s), [])
+        if force or _stale(o, [s] + hdrs, flags):
+            _make(o, [cc] + flags + ["-c", s, "-o", o], flags, verbose)
         objs.append(o)
-    if force or _stale(LIB, objs):
-        cmd = [cc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.check_call(cmd)
+    parts = [os.path.basename(o) for o in objs]
+    if force or _stale(LIB, objs, parts):
+        _make(LIB, [cc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs, parts, verbose)
     build_binding(force, verbose)
     return LIB
 
