@@ -83,3 +83,14 @@ def test_a_build_that_ends_early_goes_on_where_it_stopped(made, monkeypatch):
     monkeypatch.setattr(B.subprocess, "check_call", done)
     B.build(verbose=False)
     assert sorted(before + made) == sorted(OBJECTS + ["libsequoia_hip.so", "_paged.so"])
+
+
+def test_the_entry_compiles_each_time(made, monkeypatch):
+    import __graft_entry__ as entry
+    from sequoia_amd import native
+    monkeypatch.setattr(native, "load", lambda: None)
+    monkeypatch.setattr(native, "load_paged", lambda lib: None)
+    for _ in range(2):
+        made.clear()
+        entry.build()
+        assert sorted(made) == sorted(OBJECTS + ["libsequoia_hip.so", "_paged.so"])
