@@ -94,3 +94,27 @@ def test_the_entry_compiles_each_time(made, monkeypatch):
         made.clear()
         entry.build()
         assert sorted(made) == sorted(OBJECTS + ["libsequoia_hip.so", "_paged.so"])
+
+
+def test_without_a_host_compiler_the_library_is_built_all_the_same(made, monkeypatch, tmp_path, capsys):
+    from sequoia_amd import native
+    B.build(verbose=False)
+    run = B.subprocess.check_call
+
+    def fails(cmd):
+        if cmd[0] == "no-such-compiler":
+            raise FileNotFoundError(cmd[0])
+        run(cmd)
+
+    monkeypatch.setenv("CXX", "no-such-compiler")
+    monkeypatch.setattr(B.subprocess, "check_call", fails)
+    made.clear()
+    assert B.build(force=True, verbose=False) == B.LIB
+    assert "libsequoia_hip.so" in made and not os.path.exists(B.BINDING) and "_paged.so was not built" in capsys.readouterr().err
+    monkeypatch.setattr(native, "PAGED_PATH", B.BINDING)
+    with pytest.raises(native.SequoiaNativeError, match="not found"):
+        native.load_paged(None)
+    monkeypatch.setenv("CXX", "g++")
+    made.clear()
+    B.build(verbose=False)
+    assert made == ["_paged.so"]
