@@ -552,7 +552,8 @@ int sq_kv_read_paged(const void* k_pages, const void* v_pages, const void* k_sca
 /* Attention of the new tokens (their own rows written before): row i of sequence b sees keys [0, d_seq_lens[b] + i];
  * out [n_rows][H * D] (row stride out_stride) = softmax(scale * q k^T) v, sums in fp32.  q: element (head, row, 0) at
  * head * q_head_stride + row * q_row_stride.  max_rows / max_len: no sequence brings more rows / sees more keys (they size the
- * launch; keys beyond them are left out, rows may be).  A row that sees nothing is zeros.  scale > 0.
+ * launch; keys beyond them are left out, rows may be).  A row that sees nothing is zeros.  Where a row sees an infinity or a NaN of V, a value
+ * that the element type does not hold among them, its result is not finite.  scale > 0.
  * workspace: sq_paged_attention_workspace_bytes bytes (may be 0), free again when the call's work on the stream is done.  */
 size_t sq_paged_attention_workspace_bytes(int n_seqs, int n_rows, int max_rows, int max_len, int n_heads, int h_kv, int d);
 int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t q_row_stride, const void* k_pages, const void* v_pages,

@@ -84,10 +84,12 @@ template <typename T> __device__ __forceinline__ bool take_nonfinite(typename ve
 }
 // the four elements of a stored row of V from column d on, those that are finite as 0
 template <typename T, int D, bool Q8> __device__ __forceinline__ void hidden4(const PagedAttnParams& P, size_t row, int d, float (&x)[4]) {
-    if constexpr (Q8) {
-        const uint32_t w = *(const uint32_t*)((const uint8_t*)P.v + row * D + d);
+    if constexpr (Q8) {                             // (a code that is NaN, or one whose value T does not hold)
+        const uint32_t code = *(const uint32_t*)((const uint8_t*)P.v + row * D + d);
+        typename vec_of<T>::v8 w, none;
+        e4m3_expand<T>(u32x4{code, 0, 0, 0}, e4m3_scale(P.vs[row]), w, none);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = ((w >> (8 * j)) & 0x7fu) == 0x7fu ? NAN : 0.f;
+        for (int j = 0; j < 4; ++j) x[j] = __builtin_fabsf((float)w[j]) < INFINITY ? 0.f : (float)w[j];
     } else {
         const typename vec_of<T>::v4 w = *(const typename vec_of<T>::v4*)((const T*)P.v + row * D + d);
 #pragma unroll

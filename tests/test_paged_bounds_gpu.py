@@ -1,0 +1,59 @@
+"""The paged operators at the ends of what their arguments may hold, in every kernel of the attention: one tile of 16 and of 32 rows,
+whole and shared out; many rows, unsplit, split and shared out."""
+import math
+
+import pytest
+import torch
+
+from test_paged_gpu import DEV, Pool, run_attention
+
+pytestmark = pytest.mark.gpu
+# heads, h_kv, d, page, past, new
+KERNELS = [
+    (4, 4, 64, 16, [20, 100], [3, 2]),
+    (4, 4, 64, 16, [1400, 100], [3, 2]),
+    (8, 1, 128, 64, [37, 30], [4, 3]),
+    (8, 1, 128, 64, [37, 1500], [4, 3]),
+    (4, 4, 64, 32, [20, 10], [150, 40]),
+    (8, 2, 128, 64, [1800, 40], [40, 3]),
+    (32, 4, 64, 16, [(37 * i) % 400 + 20 for i in range(34)], [5] * 34),
+]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from sequoia_amd.ops import get_ops
+    o = get_ops()
+    assert o.name == "hip" and o.lib.sq_device_ready() == 1
+    return o
+
+
+def queries(heads, rows, d, dtype, seed=3):
+    return torch.randn((heads, rows, d), generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("heads,h_kv,d,page,past,new", KERNELS)
+def test_a_value_that_fp16_does_not_hold_reaches_who_sees_it(ops, heads, h_kv, d, page, past, new):
+    """e4m3 rows stand for code * 2^(byte - 127), whoever wrote them: 448 * 2^13 is an infinity of fp16, wherever in a sequence it
+    stands; 2^13 and smaller values beside it are not.  A result that an infinity is part of is not finite."""
+    total = [p + n for p, n in zip(past, new)]
+    for back in (1, 2):                                                  # the last stored row (everyone sees it), the chunk's second
+        pool = Pool(total, h_kv, d, page, torch.float16, True, 91)
+        codes, scales = torch.full(pool.pages[1].shape, 0x38, dtype=torch.uint8), torch.full(pool.scales[1].shape, 127, dtype=torch.uint8)
+        for b, p in enumerate(past):
+            at = p - 1 if back == 1 else p + 1
+            codes[int(pool.table[b, at // page]), :, at % page, 5] = 0x7e
+            codes[int(pool.table[b, at // page]), :, at % page, 9] = 0xfe
+            scales[int(pool.table[b, at // page]), :, at % page] = 140
+        pool.dev[1], pool.dev_scales[1] = codes.to(DEV).view(torch.float8_e4m3fn), scales.to(DEV)
+        out = run_attention(ops, pool, queries(heads, sum(new), d, torch.float16).to(DEV), past, new, d ** -0.5, max_rows=max(new), max_len=max(total))
+        out, t = out.view(-1, heads, d), 0
+        for n in new:
+            sees = torch.arange(n) >= (0 if back == 1 else 1)
+            got = out[t:t + n]
+            # (an infinity, or NaN where its weight is below what 16 bits hold beside the row's largest: 0 times an infinity)
+            assert not bool(got[sees][:, :, [5, 9]].isfinite().any())
+            assert not bool((got[sees][:, :, 5] == -math.inf).any() or (got[sees][:, :, 9] == math.inf).any())
+            others = [i for i in range(d) if i not in (5, 9)]
+            assert bool(got[~sees].isfinite().all()) and bool(got[:, :, others].isfinite().all())
+            t += n
