@@ -108,6 +108,8 @@ __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)"
 struct AttnItem {
     int seq, kvh, past, rows, first, row0, end, split, n_parts;   // packed rows of the (sequence, KV head), cu_rows[seq], first row, key end
 };
+// stored rows of sequence b, no more than the keys that count: a length of any size (a padding's marker) overflows nothing
+__device__ __forceinline__ int past_of(const PagedAttnParams& P, int length) { return length < P.max_len ? length : P.max_len; }
 __device__ __forceinline__ int attn_tile_end(const PagedAttnParams& P, int past, int rows, int tile, int tile_rows) {
     int last = (tile + 1) * tile_rows;
     last = last < rows ? last : rows;
@@ -122,7 +124,7 @@ __device__ __forceinline__ bool attn_item(const PagedAttnParams& P, int tile_row
     I.split = w % P.n_splits;
     I.first = __builtin_amdgcn_readfirstlane(P.cu_rows[I.seq]);        // scalar registers: what branches on these is uniform
     const int n = __builtin_amdgcn_readfirstlane(P.cu_rows[I.seq + 1]) - I.first;
-    I.past = __builtin_amdgcn_readfirstlane(P.seq_lens[I.seq]);
+    I.past = past_of(P, __builtin_amdgcn_readfirstlane(P.seq_lens[I.seq]));
     if (I.first < 0 || n <= 0 || n > P.n_rows - I.first) return false;      // no rows, or offsets that name none
     I.rows = n * P.group;
     I.row0 = tile * tile_rows;
@@ -167,6 +169,7 @@ template <bool UNIFORM = false> __device__ __forceinline__ Rows rows_of_seq(cons
     } else {
         R.first = P.cu_rows[b]; upto = P.cu_rows[b + 1]; R.past = P.seq_lens[b];
     }
+    R.past = past_of(P, R.past);
     const int n = upto - R.first;
     R.rows = R.first >= 0 && n > 0 && n <= P.n_rows - R.first ? n * P.group : 0;
     R.end = R.rows ? attn_tile_end(P, R.past, R.rows, 0, P.tile_rows) : 0;
@@ -870,7 +873,7 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(PagedAttnPara
     float m = there ? P.part_ml[(row + lane * step) * 2] : -INFINITY, l = there ? P.part_ml[(row + lane * step) * 2 + 1] : 0.f;
     const int seq = seq_of_row(P.cu_rows, P.n_seqs, t);
     if (seq >= P.n_seqs) return;
-    const int first = P.cu_rows[seq], n = P.cu_rows[seq + 1] - first, past = P.seq_lens[seq];
+    const int first = P.cu_rows[seq], n = P.cu_rows[seq + 1] - first, past = past_of(P, P.seq_lens[seq]);
     if (first < 0 || t < first || n > P.n_rows - first) return;
     const int rows = n * P.group, r = (t - first) * P.group + head % P.group;
     if (r >= P.n_tiles * tile_rows) return;                 // rows that were left out
@@ -919,7 +922,7 @@ __global__ void __launch_bounds__(256) paged_attention_join_rows_kernel(PagedAtt
     if (first < 0 || n > P.n_rows - first || r < 0 || r >= P.tile_rows) return;       // rows that were left out
     const int2 u = P.units[seq * P.h_kv + head / P.group];
     // a unit without keys (a length below zero) has no parts, and nobody wrote its entry: its rows are zeros
-    const bool none = attn_tile_end(P, P.seq_lens[seq], n * P.group, 0, P.tile_rows) == 0;
+    const bool none = attn_tile_end(P, past_of(P, P.seq_lens[seq]), n * P.group, 0, P.tile_rows) == 0;
     const int parts = __builtin_amdgcn_readfirstlane(none ? 0 : u.y), g0 = __builtin_amdgcn_readfirstlane(u.x);
     if (parts == 1) return;                                 // written already
     auto slot = [&](int p) { return (size_t)(p ? (g0 & ~1) + 2 * p : g0) * P.tile_rows + r; };

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+import paged_reference as R
 from test_paged_gpu import DEV, Pool, run_attention
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +58,20 @@ def test_a_value_that_fp16_does_not_hold_reaches_who_sees_it(ops, heads, h_kv, d
             others = [i for i in range(d) if i not in (5, 9)]
             assert bool(got[~sees].isfinite().all()) and bool(got[:, :, others].isfinite().all())
             t += n
+
+
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 3, 2 ** 30 + 5])
+@pytest.mark.parametrize("heads,h_kv,d,page,past,new", KERNELS)
+def test_a_length_of_any_size_sees_the_keys_that_count(ops, heads, h_kv, d, page, past, new, length):
+    """Keys from max_len on are left out, however far the length goes beyond."""
+    total = [p + n for p, n in zip(past, new)]
+    pool = Pool(total, h_kv, d, page, torch.float16, False, 92)
+    most = pool.width * page
+    keys = [torch.arange(most)] + [torch.arange(t) for t in total[1:]]
+    q = queries(heads, sum(new), d, torch.float16)
+    out, t = run_attention(ops, pool, q.to(DEV), [length] + past[1:], new, d ** -0.5, max_rows=max(new), max_len=most), 0
+    for b, n in enumerate(new):
+        k, v = (R.stored(pool.pages[i], None, pool.table[b], keys[b]) for i in (0, 1))
+        want, bound = R.attention(q[:, t:t + n].double(), k, v, past[b] if b else most, d ** -0.5, torch.float16)
+        assert bool(((out[t:t + n].view(n, heads, d).double() - want).abs() <= bound).all()), b
+        t += n
