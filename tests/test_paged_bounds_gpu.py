@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import paged_reference as R
-from test_paged_gpu import DEV, Pool, run_attention
+from test_paged_gpu import DEV, Pool, cu, i32, run_attention
 
 pytestmark = pytest.mark.gpu
 # heads, h_kv, d, page, past, new
@@ -75,3 +75,52 @@ def test_a_length_of_any_size_sees_the_keys_that_count(ops, heads, h_kv, d, page
         want, bound = R.attention(q[:, t:t + n].double(), k, v, past[b] if b else most, d ** -0.5, torch.float16)
         assert bool(((out[t:t + n].view(n, heads, d).double() - want).abs() <= bound).all()), b
         t += n
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("heads,h_kv,d,page,past,new", KERNELS)
+def test_pages_outside_the_pool(ops, heads, h_kv, d, page, past, new, quantised):
+    """Entries that name no page, in one sequence's table: its rows in front of them and the other sequences are right, nothing but the
+    rows of the batch is written, the pages stay as they are."""
+    total = [p + n for p, n in zip(past, new)]
+    pool = Pool(total, h_kv, d, page, torch.bfloat16, quantised, 93)
+    bad = -(-(past[0] + 1) // page)                                      # the first page behind the first new token's keys
+    pool.table[0, bad:] = torch.tensor([-5, 1 << 30, -(2 ** 31), pool.n_pages] * (pool.width // 4 + 1), dtype=torch.int32)[:pool.width - bad]
+    rows, cols = sum(new), heads * d
+    q = queries(heads, rows, d, torch.bfloat16)
+    guard = torch.full((rows + 4, cols + 8), 3.0, dtype=torch.bfloat16, device=DEV)
+    before = [t.view(torch.uint8).clone() for t in pool.dev]
+    ops.paged_attention(q.to(DEV), out=guard[2:2 + rows, 4:4 + cols], seq_lens=i32(past), cu_rows=cu(new).to(DEV), scale=d ** -0.5, max_rows=max(new),
+                        max_len=max(total), **pool.kw())
+    torch.cuda.synchronize()
+    for a, b in zip(pool.dev, before):
+        assert torch.equal(a.view(torch.uint8), b)
+    guard = guard.cpu()
+    out = guard[2:2 + rows, 4:4 + cols].clone()
+    guard[2:2 + rows, 4:4 + cols] = 3.0
+    assert bool((guard == 3.0).all())
+    t = 0
+    for b, (p, n) in enumerate(zip(past, new)):
+        seen = n if b else max(1, min(n, bad * page - p))                # rows whose keys all lie in front of the bad pages
+        k, v = (R.stored(pool.pages[i], pool.scales[i], pool.table[b], torch.arange(p + seen)) for i in (0, 1))
+        want, bound = R.attention(q[:, t:t + seen].double(), k, v, p, d ** -0.5, torch.bfloat16)
+        assert bool(((out[t:t + seen].view(seen, heads, d).double() - want).abs() <= bound).all()), b
+        t += n
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("heads,h_kv,d,page,past,new", KERNELS)
+def test_a_call_repeats_itself_whatever_its_workspace_held(ops, heads, h_kv, d, page, past, new, quantised):
+    """The same bits each time: the workspace comes from memory that held NaN, or zeros, or another call's sums."""
+    total = [p + n for p, n in zip(past, new)]
+    pool = Pool(total, h_kv, d, page, torch.float16, quantised, 94)
+    q = queries(heads, sum(new), d, torch.float16).to(DEV)
+    size = ops.lib.sq_paged_attention_workspace_bytes(len(new), sum(new), max(new), max(total), heads, h_kv, d)
+    want = None
+    for fill in (0, 0xff, None, 0x7f, None):
+        if size and fill is not None:
+            block = torch.full((size,), fill, dtype=torch.uint8, device=DEV)
+            del block                                                    # the next allocation of this size
+        got = run_attention(ops, pool, q, past, new, d ** -0.5, max_rows=max(new), max_len=max(total))
+        want = got if want is None else want
+        assert torch.equal(got, want)
