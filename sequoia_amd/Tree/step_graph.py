@@ -34,11 +34,11 @@ FUSE_STAGE = os.environ.get("SEQUOIA_FUSE_STAGE", "1") == "1"
 #       MLP of the last layer, no final norm, no lm_head, no row statistics: TreeContext.need_logits = False).  Committed
 #       tokens are identical by construction (the draft rows of leaves are never read); "0" runs the full forward.
 #   OVERLAP_LAST_LEVEL ("0", default): "1" additionally captures that forward on a forked stream, concurrent with the
-#       target's verify forward, joined before the verifier; "2" the same with the step captured on a high-priority stream
-#       and the fork on a low-priority one.  MEASURED NEGATIVE on MI355X (profiles/r05_overlap_last_level_not_adopted.md:
+#       target's verify forward, joined before the verifier.  MEASURED NEGATIVE on MI355X (profiles/r05_overlap_last_level_not_adopted.md:
 #       config B 5.29 -> 5.40 ms / step, config D 12.03 -> 12.22): the target's projections need all 256 CUs in ONE
 #       resident wave of workgroups, and every draft kernel that holds a CU when such a launch starts stretches its tail
-#       by more than the draft forward saves.  Kept as an opt-in for other tree / model shapes.
+#       by more than the draft forward saves.  Kept as an opt-in for other tree / model shapes.  (All streams have the
+#       default priority: work on streams of different ones has hung, and it gained nothing here, 5.35 ms / step.)
 KV_ONLY_LAST_LEVEL = os.environ.get("SEQUOIA_KV_ONLY_LAST_LEVEL", "1") == "1"
 OVERLAP_LAST_LEVEL = os.environ.get("SEQUOIA_OVERLAP_LAST_LEVEL", "0")
 
@@ -120,7 +120,7 @@ class StepState:
         n_levels = len(g["levels"])
         kv_only = KV_ONLY_LAST_LEVEL and self.cuda and getattr(dm.model, "ts", None) is not None
         # (a sharded draft runs collectives: its forward stays on the step's one stream, in the ranks' common order)
-        overlap = kv_only and OVERLAP_LAST_LEVEL in ("1", "2") and getattr(dm.model, "reduce_fn", None) is None
+        overlap = kv_only and OVERLAP_LAST_LEVEL == "1" and getattr(dm.model, "reduce_fn", None) is None
         side = None
         for li, (lv, f) in enumerate(zip(g["levels"], self.fwd_levels)):
             first = lv["first_child"]
@@ -180,7 +180,7 @@ class StepState:
 
     def _side_stream(self):
         if getattr(self, "_side", None) is None:
-            self._side = torch.cuda.Stream(device=self.device, priority=0)      # (0 = the lowest priority)
+            self._side = torch.cuda.Stream(device=self.device)
         return self._side
 
     def _stage(self, f, rel_slot0, rel_kv_len, advance=False):
@@ -230,8 +230,7 @@ class StepState:
         torch.cuda.current_stream().wait_stream(s)
         self.step[SQ_STEP_GT] = 1
         graph = torch.cuda.CUDAGraph()
-        kw = dict(stream=torch.cuda.Stream(device=self.device, priority=-1)) if OVERLAP_LAST_LEVEL == "2" else {}
-        with torch.cuda.graph(graph, capture_error_mode=capture_mode(), **kw):
+        with torch.cuda.graph(graph, capture_error_mode=capture_mode()):
             self.body()
         self.graph = graph
         for kv, off, dirty in marks:
