@@ -524,7 +524,8 @@ int sq_level_attention_f16(const void* qkv, const float* qkv_slab, int splits, i
  * sequence -- a padded batch -- are left alone).  A layer's pages are [n_pages][H_kv][page_size][D], page_size 16 / 32 / 64 /
  * 128 / 256, D 64 / 128; row j of sequence b lives in page d_page_table[b * table_width + j / page_size].  Elements are fp16 or
  * bf16 (dtype), the same for rows, tables of cosines and outputs; with k_scales and v_scales ([n_pages][H_kv][page_size] bytes)
- * the pages hold e4m3 codes (OCP, [n_pages][H_kv][page_size][D] bytes) and a row's value is code * 2^(byte - 127).
+ * the pages hold e4m3 codes (OCP, [n_pages][H_kv][page_size][D] bytes) and a row's value is code * 2^(byte - 127), rounded to
+ * the element type (which holds all but the smallest of rows of about 2^-7 (fp16) or 2^-116 (bf16) and below); bytes 1 to 254.
  * Lengths, offsets and tables are read on the device: one captured launch serves every step whose host-side bounds hold.  A
  * page number outside the pool is never followed: rows there are not written or read back, and as keys they are undefined.
  * Pages that new rows land in belong to one sequence each (two rows written to one place: one of them, or parts of both, stay).
@@ -552,8 +553,8 @@ int sq_kv_read_paged(const void* k_pages, const void* v_pages, const void* k_sca
 /* Attention of the new tokens (their own rows written before): row i of sequence b sees keys [0, d_seq_lens[b] + i];
  * out [n_rows][H * D] (row stride out_stride) = softmax(scale * q k^T) v, sums in fp32.  q: element (head, row, 0) at
  * head * q_head_stride + row * q_row_stride.  max_rows / max_len: no sequence brings more rows / sees more keys (they size the
- * launch; keys beyond them are left out, rows may be).  A row that sees nothing is zeros.  Where a row sees an infinity or a NaN of V, a value
- * that the element type does not hold among them, its result is not finite.  scale > 0.
+ * launch; keys beyond them are left out, rows may be).  A row that sees nothing is zeros.  Where a row sees an
+ * infinity or a NaN of V, a value that the element type does not hold among them, its result is not finite.  scale > 0.
  * workspace: sq_paged_attention_workspace_bytes bytes (may be 0), free again when the call's work on the stream is done.  */
 size_t sq_paged_attention_workspace_bytes(int n_seqs, int n_rows, int max_rows, int max_len, int n_heads, int h_kv, int d);
 int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t q_row_stride, const void* k_pages, const void* v_pages,
@@ -567,7 +568,7 @@ int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t q_row_strid
  * draft_logits: >= n_drafts, fp16 / bf16 / fp32).  With p = softmax(target / T), q = softmax(draft / T): tokens are accepted
  * while u_accept[token] * q(token) < p(token); next = the first token whose running mass of max(p - q, 0) (of p behind the last
  * drafted token, and where p is nowhere above q) exceeds u_next[b] times its total.  d_temperature[b] (NULL: `temperature`)
- * = 0: greedy, p is the first maximum.  d_n_accepted[b] = accepted tokens; d_next_tokens[b] = -1 where the deciding row is no
+ * not > 0: greedy, p is the first maximum; infinite: the largest finite number.  d_n_accepted[b] = accepted tokens; d_next_tokens[b] = -1 where the deciding row is no
  * distribution (NaN, +inf, or nothing above -inf).  A drafted token outside the vocabulary is never accepted.  Sums, probabilities and
  * running masses are 64-bit.                                                                                           */
 size_t sq_verify_drafts_workspace_bytes(int n_seqs, int n_drafts, int vocab);

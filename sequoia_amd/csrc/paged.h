@@ -4,9 +4,11 @@
 // the static slab, so a 16-row tile of keys never straddles two pages.  Row j of sequence b lives in page
 // table[b][j >> shift], row j & (P - 1).
 //
-// An e4m3 row keeps one exponent byte x: value = code * 2^(x - 127).  The scale is a power of two so that both directions are
-// exact but for the ONE rounding to e4m3's four significant bits (at most 2^-4 relative, 2^(x - 137) absolute below the
-// format's normal range): x / scale and code * scale never round, and every reader gets the same value.
+// An e4m3 row keeps one exponent byte x: value = code * 2^(x - 127).  The scale is a power of two so that what is lost is the ONE
+// rounding to e4m3's four significant bits (at most 2^-4 relative, 2^(x - 137) absolute below the format's normal range): dividing by
+// it never rounds, and multiplying by it only where the element type ends -- the smallest codes of fp16 rows of at most 448 * 2^-16
+// (0.007), whose steps lie under fp16's own of 2^-24, and of bf16 rows of 2^-116; values above the type's largest are infinities,
+// which the writer leaves none of.  Every reader of a type gets the same value.
 #pragma once
 #include "common.h"
 
@@ -64,7 +66,7 @@ __device__ __forceinline__ int seq_of_row(const int32_t* cu_rows, int n_seqs, in
     return n_seqs;
 }
 
-// 16 codes -> 16 values of T, exact: v_cvt_scalef32 multiplies by the power of two while it widens
+// 16 codes -> 16 values of T, rounded only where T ends: v_cvt_scalef32 multiplies by the power of two while it widens
 template <typename T>
 __device__ __forceinline__ void e4m3_expand(u32x4 codes, float scale, typename vec_of<T>::v8& lo, typename vec_of<T>::v8& hi) {
     typename vec_of<T>::v2 p[8];

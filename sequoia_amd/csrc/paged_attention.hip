@@ -1,9 +1,10 @@
 // Attention of a ragged batch's new tokens over a paged KV cache (their own rows already written): for sequence b with `past`
 // stored rows and n new ones, row i attends keys [0, past + i],
 //     o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   s_j = scale * q . k_j,
-// in one pass over the keys with a running maximum and sum in fp32; weights are rounded to the element type once, for the
-// second matrix product, and the sum is taken of the rounded ones.  The query heads that share a KV head are packed into the same rows of a tile (row r = token r / group,
-// head r % group), so that every stored row is read once for all of them.
+// in one pass over the keys with a running maximum and sum in fp32.  Weights are rounded to the element type once, because the matrix
+// instructions take both operands of the second product so, and the sum is taken of the rounded ones: a result is off by at most half a
+// step of the type times sum_j w_j |v_j - o|, beside half a step of its own.  The query heads that share a KV head are packed into the
+// same rows of a tile (row r = token r / group, head r % group), so that every stored row is read once for all of them.
 #include "paged.h"
 #include "attn_map.h"
 

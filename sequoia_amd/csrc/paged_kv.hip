@@ -22,9 +22,10 @@ struct PagedWriteParams {
 // of its row, so the rotation (o1 = x1 cos - x2 sin, o2 = x2 cos + x1 sin) is lane-local and a row's largest magnitude takes
 // log2(D / 16) lane exchanges.  The products of two 16-bit values are exact in fp32; the one rounding of the sum is followed by
 // the one to the stored type.
-// Bound by bytes, read once and written once, and by latency below about a hundred rows: 6000 rows of 64 + 2 * 8 heads of 128, fp16,
-// 51 us (5.5 TB/s, a large copy here reaches 5.1); 32 rows into e4m3 pages 3.6 us, a call 4.4.  The stores go past
-// the caches: cached ones took 55.6 us, and the attention that reads the rows next, mostly on another XCD, takes the same time.
+// Bound by bytes, read once and written once, and by latency below about a hundred rows: 6730 rows of 64 + 2 * 8 heads of 128, fp16,
+// 51 us (5.5 TB/s, a large copy here reaches 5.1; 42 where the call before read the same rows, which the last-level cache then holds in
+// part); 32 rows into e4m3 pages 3.6 us, a call 4.4.  The stores go past the caches: cached ones took 55.6 us, and the attention that
+// reads the rows next, mostly on another XCD, takes the same time.
 template <typename T, int D, bool Q8>
 __global__ void __launch_bounds__(PKV_THREADS) rope_kv_write_paged_kernel(PagedWriteParams P) {
     typedef typename vec_of<T>::v8 v8;

@@ -404,7 +404,8 @@ class HipOps:
         """Attention of a ragged batch's new tokens (written before by rope_kv_write_paged): row cu_rows[b] + i of q [H, n_rows, D]
         sees keys [0, seq_lens[b] + i] of sequence b; out [n_rows, H D].  max_rows / max_len: no sequence brings more rows / ends
         behind more keys (defaults and caps: n_rows, the table's whole width); they size the launch; keys beyond them are left out, rows
-        may be.  The default max_len costs workgroups that find nothing to do."""
+        may be.  The default max_len costs workgroups that find nothing to do.  A call is planned by the sequence with the most rows: a
+        prompt's chunk beside sequences of single tokens takes less time in a call of its own."""
         self._paged.attention(q, k_pages, v_pages, out, page_table, seq_lens, cu_rows, scale, max_rows, max_len, k_scales, v_scales)
         return out
 
@@ -413,7 +414,7 @@ class HipOps:
         cu_drafts[b + 1]]; target_logits [>= drafts + sequences, V] row cu_drafts[b] + b + i judges its token i and the row behind its
         last one follows, draft_logits [>= drafts, V] are the rows the tokens were drawn from.  Tokens are accepted while
         u_accept q(token) < p(token); then the next token is drawn with u_next[b] from max(p - q, 0), or from p behind the last one.
-        temperature: a number or a float32 tensor [sequences]; 0 is greedy.  n_accepted int32 / next_tokens int64 [sequences]
+        temperature: a number >= 0 or a float32 tensor [sequences], of any size; 0 is greedy.  n_accepted int32 / next_tokens int64 [sequences]
         (-1: the deciding row is no distribution)."""
         self._paged.verify(target_logits, draft_logits, draft_tokens, cu_drafts, u_accept, u_next, temperature, n_accepted, next_tokens)
         return n_accepted, next_tokens
