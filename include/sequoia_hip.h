@@ -568,9 +568,9 @@ int sq_paged_attention(const void* q, int64_t q_head_stride, int64_t q_row_strid
  * draft_logits: >= n_drafts, fp16 / bf16 / fp32).  With p = softmax(target / T), q = softmax(draft / T): tokens are accepted
  * while u_accept[token] * q(token) < p(token); next = the first token whose running mass of max(p - q, 0) (of p behind the last
  * drafted token, and where p is nowhere above q) exceeds u_next[b] times its total.  d_temperature[b] (NULL: `temperature`)
- * not > 0: greedy, p is the first maximum; infinite: the largest finite number.  d_n_accepted[b] = accepted tokens; d_next_tokens[b] = -1 where the deciding row is no
- * distribution (NaN, +inf, or nothing above -inf).  A drafted token outside the vocabulary is never accepted.  Sums, probabilities and
- * running masses are 64-bit.                                                                                           */
+ * not > 0: greedy, p is the first maximum; infinite: the largest finite number.  d_n_accepted[b] = accepted tokens;
+ * d_next_tokens[b] = -1 where the deciding row is no distribution (NaN, +inf, or nothing above -inf).  A drafted token outside the
+ * vocabulary is never accepted.  Differences of logits, sums, probabilities and running masses are 64-bit.                */
 size_t sq_verify_drafts_workspace_bytes(int n_seqs, int n_drafts, int vocab);
 int sq_verify_drafts(const void* target_logits, int64_t ld_target, const void* draft_logits, int64_t ld_draft,
                      const int64_t* d_draft_tokens, const int32_t* d_cu_drafts, int n_seqs, int n_drafts, int vocab,
